@@ -69,6 +69,21 @@ int smem_limit(PerDevice& once, Kernel* kernel, int bytes, const char* what) {
       what);
 }
 
+// Checks of a paged key/value pool [pages, kv_heads, page_size, head_dim] (page stride in elements, everything
+// below it dense) and of the page table's shape; the same rules for every entry point that takes one.
+inline int check_pool(const char* name, int64_t page_stride, int64_t pages, int64_t page_size, int64_t kv_heads,
+                      int64_t head_dim, int64_t table_stride, int64_t table_rows, int64_t table_columns) {
+  if (pages < 1 || pages > 2147483647 || kv_heads < 1 || kv_heads > 1024)
+    return fail(Q3T_EINVAL, "%s: invalid pool", name);
+  if (page_size < 16 || page_size > 65536 || page_size % 16)
+    return fail(Q3T_EUNSUPPORTED, "%s: page_size must be a multiple of 16 within 16..65536", name);
+  if (page_stride < kv_heads * page_size * head_dim || page_stride % 8 || page_stride > (int64_t(1) << 40))
+    return fail(Q3T_EINVAL, "%s: page stride", name);
+  if (table_rows < 1 || table_columns < 1 || table_columns > 2147483647 || (table_rows > 1 && table_stride < table_columns))
+    return fail(Q3T_EINVAL, "%s: invalid page table", name);
+  return Q3T_OK;
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -7,6 +7,7 @@ written, as the reference wrappers do.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Optional
@@ -516,6 +517,169 @@ def decode_attention_qkv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin_
          keys.data_ptr(), values.data_ptr(), positions.data_ptr(), out.data_ptr(), rows, q_heads, kv_heads, head_dim,
          n_slots, capacity, context, float(scale), ws.data_ptr(), ws.numel(), status_word(qkv.device).data_ptr(),
          _stream())
+    return out
+
+
+# ------------------------------------------------------------------ paged key/value cache
+def _on(device: torch.device):
+    """The context in which to launch on `device`: the current one, or a switch to another GPU."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _check_paged(what: str, rows, key_pages, value_pages, page_table, **int64s) -> None:
+    """The checks that the paged operators share: `rows` is their bf16 input, int64s their index vectors."""
+    tensors = (rows, key_pages, value_pages, page_table, *int64s.values())
+    _need_cuda(*tensors)
+    device = rows.device
+    if any(t is not None and t.device != device for t in tensors):
+        raise ValueError(f"{what}: tensors must be on one device")
+    if (key_pages.ndim != 4 or key_pages.shape != value_pages.shape or key_pages.dtype != BF16
+            or value_pages.dtype != BF16 or rows.dtype != BF16):
+        raise ValueError(f"{what}: expected BF16 rows and BF16 key and value pages [pages, Hkv, page_size, D]")
+    _, _, size, dim = key_pages.shape
+    stride = key_pages.stride()
+    if stride != value_pages.stride() or stride[1:] != (size * dim, dim, 1):
+        raise ValueError(f"{what}: pages must be dense [Hkv, page_size, D] blocks with one page stride")
+    if page_table.ndim != 2 or page_table.dtype != torch.int32 or page_table.stride(1) != 1:
+        raise ValueError(f"{what}: page table must be INT32 [sequences, columns] with unit inner stride")
+    for name, t in int64s.items():
+        if t is not None and (t.dtype != torch.int64 or t.ndim != 1 or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous INT64 vector")
+
+
+def _check_query(what: str, query, key_pages, out) -> None:
+    if (query.ndim != 3 or query.shape[2] != key_pages.shape[3] or query.stride(2) != 1
+            or query.stride(1) != query.shape[2] or query.shape[1] % key_pages.shape[1]):
+        raise ValueError(f"{what}: query must be [rows, Hq, D] with dense rows, Hq a multiple of Hkv")
+    if out is not None and (out.shape != query.shape or out.dtype != BF16 or not out.is_contiguous()
+                            or out.device != query.device):
+        raise ValueError(f"{what}: out must be contiguous BF16 shaped like query")
+
+
+def paged_qk_norm_rope_kv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin_table, rotary_positions,
+                          cache_positions, page_table, key_pages, value_pages, *, q_heads, kv_heads, head_dim,
+                          sequences=None, query_out=None):
+    """Per-head q/k RMSNorm, RoPE and the paged K/V write of packed QKV rows (q3t_paged_qk_norm_rope_kv).
+
+    qkv BF16 [rows, (q_heads + 2 * kv_heads) * head_dim] (rows may be strided); cos/sin tables BF16
+    [positions, head_dim], indexed by rotary_positions; key_pages / value_pages BF16 [pages, kv_heads,
+    page_size, head_dim]; page_table INT32 [sequences, columns]. Row r writes position cache_positions[r] of
+    sequence sequences[r] (None: of sequence r); rows with a negative sequence are skipped. No two rows may
+    write the same position of a page. Returns the queries [rows, q_heads, head_dim]."""
+    what = "paged_qk_norm_rope_kv"
+    _check_paged(what, qkv, key_pages, value_pages, page_table, rotary_positions=rotary_positions,
+                 cache_positions=cache_positions, sequences=sequences)
+    pages, heads, size, dim = key_pages.shape
+    if (qkv.ndim != 2 or qkv.stride(1) != 1 or heads != kv_heads or dim != head_dim
+            or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim):
+        raise ValueError(f"{what}: qkv must be [rows, (q + 2 kv) * head_dim] with unit inner stride")
+    rows = qkv.shape[0]
+    if any(t is not None and t.shape[0] != rows for t in (rotary_positions, cache_positions, sequences)):
+        raise ValueError(f"{what}: positions and sequences must have one entry per row")
+    if sequences is None and page_table.shape[0] < rows:
+        raise ValueError(f"{what}: page table must have a row per qkv row")
+    for t, shape in ((q_norm_weight, (dim,)), (k_norm_weight, (dim,)), (cos_table, (cos_table.shape[0], dim)),
+                     (sin_table, (cos_table.shape[0], dim))):
+        if t is not None and (t.device != qkv.device or t.dtype != BF16 or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"{what}: norm weights [head_dim] and cos/sin tables [positions, head_dim] must be "
+                             "contiguous BF16")
+    if query_out is None:
+        query_out = torch.empty(rows, q_heads, dim, dtype=BF16, device=qkv.device)
+    elif (query_out.shape != (rows, q_heads, dim) or query_out.dtype != BF16 or not query_out.is_contiguous()
+          or query_out.device != qkv.device):
+        raise ValueError(f"{what}: query_out must be contiguous BF16 [rows, q_heads, head_dim]")
+    if rows == 0:
+        return query_out
+    with _on(qkv.device):
+        call("q3t_paged_qk_norm_rope_kv", qkv.data_ptr(), qkv.stride(0), _ptr(q_norm_weight), _ptr(k_norm_weight),
+             float(eps), cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0], rotary_positions.data_ptr(),
+             cache_positions.data_ptr(), _ptr(sequences), page_table.data_ptr(), page_table.stride(0),
+             page_table.shape[0], page_table.shape[1], query_out.data_ptr(), key_pages.data_ptr(),
+             value_pages.data_ptr(), key_pages.stride(0), pages, size, rows, q_heads, kv_heads, dim,
+             status_word(qkv.device).data_ptr(), _stream())
+    return query_out
+
+
+def _paged_workspace(what: str, need: int, workspace, device):
+    """The caller's workspace, or one of this call's own: calls and captured graphs never share it unasked."""
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be a contiguous tensor on the query's device")
+    return workspace
+
+
+def paged_decode_attention_workspace_bytes(rows, q_heads, kv_heads, head_dim, context) -> int:
+    return int(_lib.load().q3t_paged_decode_attention_workspace_bytes(rows, q_heads, kv_heads, head_dim, context))
+
+
+def paged_decode_attention(query, key_pages, value_pages, page_table, positions, *, context=None, scale=None, out=None,
+                           workspace: Optional[torch.Tensor] = None):
+    """Attention of one new token per sequence over a paged cache (q3t_paged_decode_attention).
+
+    Query row r [Hq, D] (rows may be strided) sees keys 0 .. positions[r] of sequence r, whose pages
+    page_table[r] names; positions[r] = -1 sees none and gives zeros. `context`: a bound that no position
+    reaches (default: what the table can hold). `out` must not overlap query or pages. `workspace`: a buffer
+    of paged_decode_attention_workspace_bytes that no other call uses meanwhile; by default the call takes its own."""
+    what = "paged_decode_attention"
+    _check_paged(what, query, key_pages, value_pages, page_table, positions=positions)
+    _check_query(what, query, key_pages, out)
+    pages, kv_heads, size, dim = key_pages.shape
+    rows, q_heads, _ = query.shape
+    if positions.shape[0] != rows or page_table.shape[0] < rows:
+        raise ValueError(f"{what}: one position and a page table row per query row")
+    context = page_table.shape[1] * size if context is None else int(context)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    out = torch.empty(query.shape, dtype=BF16, device=query.device) if out is None else out
+    if rows == 0:
+        return out
+    with _on(query.device):
+        ws = _paged_workspace(what, paged_decode_attention_workspace_bytes(rows, q_heads, kv_heads, dim, context),
+                              workspace, query.device)
+        call("q3t_paged_decode_attention", query.data_ptr(), query.stride(0), key_pages.data_ptr(),
+             value_pages.data_ptr(), key_pages.stride(0), pages, size, page_table.data_ptr(), page_table.stride(0),
+             page_table.shape[1], positions.data_ptr(), out.data_ptr(), rows, q_heads, kv_heads, dim, context, scale,
+             _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(), status_word(query.device).data_ptr(),
+             _stream())
+    return out
+
+
+def paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, head_dim, context) -> int:
+    return int(_lib.load().q3t_paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, head_dim,
+                                                                       context))
+
+
+def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offsets, start_positions, *, out,
+                            scale=None, workspace: Optional[torch.Tensor] = None):
+    """Causal attention of packed prompts over a paged cache (q3t_paged_prefill_attention).
+
+    Sequence s owns query rows row_offsets[s] .. row_offsets[s + 1] - 1; its i-th row has position
+    start_positions[s] + i (start > 0: a chunk after a cached prefix; negative positions are left padding and
+    give zeros) and sees keys 0 .. that position in the pages of page_table[s], which hold them already. Rows
+    that no sequence owns are left as they are in `out`. `workspace`: as for paged_decode_attention."""
+    what = "paged_prefill_attention"
+    _check_paged(what, query, key_pages, value_pages, page_table, row_offsets=row_offsets,
+                 start_positions=start_positions)
+    _check_query(what, query, key_pages, out)
+    pages, kv_heads, size, dim = key_pages.shape
+    rows, q_heads, _ = query.shape
+    sequences = start_positions.shape[0]
+    if row_offsets.shape[0] != sequences + 1 or page_table.shape[0] < sequences:
+        raise ValueError(f"{what}: sequences + 1 row offsets and a page table row per start position")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if rows == 0 or sequences == 0:
+        return out
+    with _on(query.device):
+        need = paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, dim,
+                                                       page_table.shape[1] * size)
+        ws = _paged_workspace(what, need, workspace, query.device)
+        call("q3t_paged_prefill_attention", query.data_ptr(), query.stride(0), key_pages.data_ptr(),
+             value_pages.data_ptr(), key_pages.stride(0), pages, size, page_table.data_ptr(), page_table.stride(0),
+             page_table.shape[1], row_offsets.data_ptr(), start_positions.data_ptr(), sequences, out.data_ptr(), rows,
+             q_heads, kv_heads, dim, scale, _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(),
+             status_word(query.device).data_ptr(), _stream())
     return out
 
 

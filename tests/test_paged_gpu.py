@@ -1,0 +1,456 @@
+"""The paged key/value cache operators against plain 64-bit forms: the page write, the attention of one new token
+and the causal attention of packed prompts, alone, together and in captured graphs."""
+import pytest
+import torch
+
+from tests.paged_reference import BF16, Case, assert_within, attend, rng, tables, turn
+
+pytestmark = pytest.mark.gpu
+
+# q heads, kv heads, head dim: the talker's, the codec transformer's, and groups of 1, 3, 4, 7, 8, 9 and 16
+GEOMETRIES = [(16, 8, 128), (8, 8, 64), (12, 4, 64), (8, 2, 128), (14, 2, 64), (8, 1, 128), (9, 1, 128), (16, 1, 64)]
+PAGES = [16, 48, 64, 256]
+
+
+@pytest.fixture(scope="module")
+def ops(cuda):
+    from qwen3_tts_b200 import ops as _ops
+    return _ops
+
+
+def rows_of(shape, seed, strided):
+    rows, width = shape[0], shape[1] * shape[2] if len(shape) == 3 else shape[1]
+    x = torch.randn(rows, width + (40 if strided else 0), generator=rng(seed)).to(BF16)
+    return x[:, :width].unflatten(1, shape[1:]) if len(shape) == 3 else x[:, :width]
+
+
+def on(x, device):
+    """x on the device, its strides kept."""
+    if x.is_contiguous():
+        return x.to(device)
+    whole = torch.as_strided(x, (x.shape[0], x.stride(0)), (x.stride(0), 1))
+    return torch.as_strided(whole.to(device), x.shape, x.stride())
+
+
+# ------------------------------------------------------------------ the write
+def check_write(ops, cuda, q, kv, d, page, lengths, *, new, norm, strided, one_pool=False, seed=0):
+    case = Case(lengths, kv, d, page, seed=seed, one_pool=one_pool)
+    if new:   # the last position of every sequence
+        at, seq = torch.tensor(lengths) - 1, None
+    else:     # every position of every sequence, in a shuffled order
+        at = torch.cat([torch.arange(n) for n in lengths])
+        seq = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths))
+        order = torch.randperm(len(at), generator=rng(seed + 1))
+        at, seq = at[order], seq[order]
+    rows = len(at)
+    qkv = rows_of((rows, (q + 2 * kv) * d), seed + 2, strided)
+    weights = [(1 + 0.2 * torch.randn(d, generator=rng(seed + 3 + i))).to(BF16) if norm else None for i in range(2)]
+    cos, sin = tables(max(lengths) + 5, d)
+    rotary = at + 4
+    keys, values, table = case.to(cuda)
+    dev = [None if t is None else t.to(cuda) for t in (*weights, cos, sin, rotary, at, seq)]
+    got = ops.paged_qk_norm_rope_kv(on(qkv, cuda), dev[0], dev[1], 1e-6, dev[2], dev[3], dev[4], dev[5], table, keys,
+                                    values, q_heads=q, kv_heads=kv, head_dim=d, sequences=dev[6])
+    assert ops.read_status(cuda) == 0
+    x = qkv.reshape(rows, q + 2 * kv, d)
+    want, bound = turn(x[:, :q], weights[0], cos[rotary], sin[rotary], 1e-6)
+    assert_within(got, want, bound, "queries")
+    want, bound = turn(x[:, q:q + kv], weights[1], cos[rotary], sin[rotary], 1e-6)
+    where = case.table[torch.arange(rows) if seq is None else seq, at // page].long()
+    assert_within(keys.cpu()[where, :, at % page], want, bound, "keys")
+    assert torch.equal(values.cpu()[where, :, at % page], x[:, q + kv:])
+    for pool, before in ((keys.cpu(), case.keys.clone()), (values.cpu(), case.values.clone())):
+        pool[where, :, at % page] = 0
+        before[where, :, at % page] = 0
+        assert torch.equal(pool.view(torch.int16), before.view(torch.int16))  # nothing else is touched
+
+
+@pytest.mark.parametrize("q,kv,d", GEOMETRIES)
+@pytest.mark.parametrize("new", [True, False])
+def test_write_heads(ops, cuda, q, kv, d, new):
+    check_write(ops, cuda, q, kv, d, 32, [1, 31, 32, 33, 70], new=new, norm=True, strided=False)
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("norm,strided,one_pool", [(True, True, False), (False, False, True), (False, True, True)])
+def test_write_pages_strides_and_rows_without_norm(ops, cuda, page, norm, strided, one_pool):
+    check_write(ops, cuda, 16, 8, 128, page, [5, 17, page, page + 1, 3 * page], new=False, norm=norm, strided=strided,
+                one_pool=one_pool)
+
+
+@pytest.mark.parametrize("count", [1, 2, 64, 257])
+def test_write_step_batches(ops, cuda, count):
+    check_write(ops, cuda, 16, 8, 128, 16, [1 + 7 * i % 60 for i in range(count)], new=True, norm=True, strided=False,
+                seed=count)
+
+
+def write_args(ops, cuda, rows=3, q=4, kv=2, d=64, page=16, columns=2):
+    table = torch.arange(rows * columns, dtype=torch.int32, device=cuda).view(rows, columns)
+    cos, sin = (t.to(cuda) for t in tables(64, d))
+    qkv = torch.randn(rows, (q + 2 * kv) * d, generator=rng(9)).to(BF16).to(cuda)
+    pool = [torch.zeros(rows * columns, kv, page, d, dtype=BF16, device=cuda) for _ in range(2)]
+    return qkv, cos, sin, table, pool
+
+
+def test_write_skips_padding_rows_and_flags_bad_positions(ops, cuda):
+    qkv, cos, sin, table, (keys, values) = write_args(ops, cuda)
+    out = torch.full((3, 4, 64), 7.0, dtype=BF16, device=cuda)
+
+    def write(at, sequences, rotary=(1, 1, 1), page_table=table):
+        keys.zero_(), values.zero_(), out.fill_(7.0)
+        ops.paged_qk_norm_rope_kv(qkv, None, None, 1e-6, cos, sin, torch.tensor(rotary, device=cuda),
+                                  torch.tensor(at, device=cuda), page_table, keys, values, q_heads=4, kv_heads=2,
+                                  head_dim=64, sequences=torch.tensor(sequences, device=cuda), query_out=out)
+        written = values.ne(0).any(-1).any(1).nonzero().tolist()
+        return written, out.ne(7.0).flatten(1).any(1).tolist(), ops.read_status(cuda)
+
+    assert write((3, 4, 5), (0, -1, 2)) == ([[0, 3], [4, 5]], [True, False, True], 0)
+    assert write((3, 1 << 40, 5), (0, -(1 << 60), 2), rotary=(1, -5, 1)) == ([[0, 3], [4, 5]], [True, False, True], 0)
+    assert write((3, 32, 5), (0, 1, 2)) == ([[0, 3], [4, 5]], [True] * 3, 8)      # past the table's columns
+    assert write((3, -1, 5), (0, 1, 2)) == ([[0, 3], [4, 5]], [True] * 3, 8)
+    assert write((3, 4, 5), (0, 3, 2)) == ([[0, 3], [4, 5]], [True] * 3, 8)       # past the table's rows
+    assert write((3, 4, 5), (0, 1, 2), rotary=(1, 64, 1)) == ([[0, 3], [2, 4], [4, 5]], [True] * 3, 8)
+    bad = table.clone()
+    bad[1, 0] = 6
+    assert write((3, 4, 5), (0, 1, 2), page_table=bad) == ([[0, 3], [4, 5]], [True] * 3, 8)
+    bad[1, 0] = -1
+    assert write((3, 20, 5), (0, 1, 2), page_table=bad) == ([[0, 3], [3, 4], [4, 5]], [True] * 3, 0)
+
+
+# ------------------------------------------------------------------ one new token
+def check_decode(ops, cuda, q, kv, d, page, lengths, *, strided=False, one_pool=False, seed=0, scale=None, context=None,
+                 columns=None, share=0, gain=1.0):
+    case = Case(lengths, kv, d, page, seed=seed, one_pool=one_pool, columns=columns, share=share)
+    query = (gain * rows_of((len(lengths), q, d), seed + 1, strided)) if not strided else \
+        rows_of((len(lengths), q, d), seed + 1, strided)
+    keys, values, table = case.to(cuda)
+    got = ops.paged_decode_attention(on(query, cuda), keys, values, table, (torch.tensor(lengths) - 1).to(cuda),
+                                     scale=scale, context=context)
+    assert ops.read_status(cuda) == 0
+    for r, n in enumerate(lengths):
+        want, bound = attend(query[r], *case.sequence(r, n), d ** -0.5 if scale is None else scale)
+        assert_within(got[r], want, bound, f"row {r} of {n} keys")
+
+
+@pytest.mark.parametrize("q,kv,d", GEOMETRIES)
+def test_decode_heads(ops, cuda, q, kv, d):
+    check_decode(ops, cuda, q, kv, d, 32, [1, 0, 15, 16, 17, 31, 32, 33, 127, 128, 129, 400])
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("strided,one_pool", [(True, False), (False, True)])
+def test_decode_pages_and_strides(ops, cuda, page, strided, one_pool):
+    check_decode(ops, cuda, 16, 8, 128, page, [page - 1, page, page + 1, 5 * page + 3], strided=strided,
+                 one_pool=one_pool, columns=9)
+
+
+@pytest.mark.parametrize("lengths", [[1], [0], [0, 0, 0], [4097], [1, 8000, 1], [3000] + [5] * 40, [513] * 70])
+@pytest.mark.parametrize("q,kv,d", [(16, 8, 128), (16, 1, 64)])
+def test_decode_lengths(ops, cuda, lengths, q, kv, d):
+    check_decode(ops, cuda, q, kv, d, 64, lengths)
+
+
+def test_decode_long_context(ops, cuda):
+    check_decode(ops, cuda, 8, 2, 128, 128, [70001, 1, 33333])
+
+
+@pytest.mark.parametrize("count", [300, 1500])
+def test_decode_many_rows(ops, cuda, count):
+    check_decode(ops, cuda, 4, 2, 64, 16, [(37 * i) % 90 for i in range(count)], seed=count)
+
+
+def test_decode_context_bound_shared_pages_and_scale(ops, cuda):
+    check_decode(ops, cuda, 16, 8, 128, 16, [90, 41, 64, 3], share=2, context=90, columns=40)
+    check_decode(ops, cuda, 16, 8, 128, 16, [90, 41, 64, 3], scale=0.5)       # peaked weights
+    check_decode(ops, cuda, 16, 8, 128, 16, [90, 41, 64, 3], scale=-0.25)
+    check_decode(ops, cuda, 16, 8, 128, 16, [90, 41, 64, 3], scale=0.0)
+
+
+def test_decode_rising_scores_move_the_reference(ops, cuda):
+    """Scores that grow by far more than the lazy margin from step to step, up and down again."""
+    n, d = 300, 64
+    case = Case([n], 1, d, 16)
+    keys, _ = case.sequence(0, n)
+    ramp = torch.cat((torch.arange(200.0), torch.arange(100.0).flip(0)))
+    for j in range(n):
+        case.keys[case.table[0, j // 16], 0, j % 16] = torch.full((d,), ramp[j].item() / 8).to(BF16)
+    query = torch.ones(1, 2, d, dtype=BF16)
+    query[0, 1] = -1
+    k, v, table = case.to(cuda)
+    got = ops.paged_decode_attention(query.to(cuda), k, v, table, torch.tensor([n - 1], device=cuda))
+    want, bound = attend(query[0], *case.sequence(0, n), d ** -0.5)
+    assert_within(got[0], want, bound)
+
+
+def test_decode_infinite_scores_follow_the_formula(ops, cuda):
+    """A key of -inf has weight 0 wherever it stands; only -inf scores, or one of +inf, have no value."""
+    n, d = 40, 64
+    for where in (0, 5, 39):
+        case = Case([n], 1, d, 16)
+        case.keys[case.table[0, where // 16], 0, where % 16, 0] = -float("inf")
+        query = torch.ones(1, 1, d, dtype=BF16)
+        k, v, table = case.to(cuda)
+        got = ops.paged_decode_attention(query.to(cuda), k, v, table, torch.tensor([n - 1], device=cuda))
+        rest = [j for j in range(n) if j != where]
+        keys, values = case.sequence(0, n)
+        want, bound = attend(query[0], keys[:, rest], values[:, rest], d ** -0.5)
+        assert_within(got[0], want, bound)
+        got = ops.paged_decode_attention(-query.to(cuda), k, v, table, torch.tensor([n - 1], device=cuda))
+        assert got.isnan().all()
+    case.keys[..., 0] = -float("inf")
+    k, v, table = case.to(cuda)
+    got = ops.paged_decode_attention(query.to(cuda), k, v, table, torch.tensor([n - 1], device=cuda))
+    assert got.isnan().all()
+
+
+def test_decode_flags_bad_positions_and_pages(ops, cuda):
+    """The row with the bad index is unspecified; its neighbours are right and nothing faults."""
+    lengths = [40, 40, 40]
+    case = Case(lengths, 8, 128, 16)
+    query = rows_of((3, 16, 128), 1, False)
+    keys, values, table = case.to(cuda)
+
+    def decode(positions, page_table=table):
+        got = ops.paged_decode_attention(query.to(cuda), keys, values, page_table, torch.tensor(positions, device=cuda))
+        for r in (0, 2):
+            assert_within(got[r], *attend(query[r], *case.sequence(r, 40), 128 ** -0.5))
+        return ops.read_status(cuda)
+
+    assert decode((39, 39, 39)) == 0
+    assert decode((39, -2, 39)) == 8
+    for entry in (len(case.keys), -1, -(1 << 31), (1 << 31) - 1):
+        bad = table.clone()
+        bad[1, 1] = entry
+        assert decode((39, 39, 39), bad) == 8
+        assert decode((39, 15, 39), bad) == 0  # the entry is not needed
+
+
+def test_decode_clamps_a_position_past_the_context(ops, cuda):
+    case = Case([64, 64], 8, 128, 16)
+    query = rows_of((2, 16, 128), 1, False)
+    keys, values, table = case.to(cuda)
+    got = ops.paged_decode_attention(query.to(cuda), keys, values, table, torch.tensor([64, 20], device=cuda))
+    assert ops.read_status(cuda) == 8
+    assert_within(got[0], *attend(query[0], *case.sequence(0, 64), 128 ** -0.5))
+    assert_within(got[1], *attend(query[1], *case.sequence(1, 21), 128 ** -0.5))
+
+
+def test_decode_repeats_bit_for_bit(ops, cuda):
+    case = Case([5000, 77, 1234, 1], 8, 128, 64)
+    query = rows_of((4, 16, 128), 1, False).to(cuda)
+    keys, values, table = case.to(cuda)
+    at = torch.tensor([4999, 76, 1233, 0], device=cuda)
+    first = ops.paged_decode_attention(query, keys, values, table, at)
+    for _ in range(20):
+        assert torch.equal(ops.paged_decode_attention(query, keys, values, table, at), first)
+
+
+# ------------------------------------------------------------------ packed prompts
+def check_prompt(ops, cuda, q, kv, d, page, counts, starts, *, lead=0, tail=0, strided=False, one_pool=False, seed=0,
+                 scale=None, columns=None):
+    lengths = [max(0, n + s) if n else max(0, s) for n, s in zip(counts, starts)]
+    case = Case(lengths, kv, d, page, seed=seed, one_pool=one_pool, columns=columns)
+    rows = lead + sum(counts) + tail
+    query = rows_of((rows, q, d), seed + 1, strided)
+    offsets = torch.tensor([lead + sum(counts[:i]) for i in range(len(counts) + 1)])
+    keys, values, table = case.to(cuda)
+    out = torch.full((rows, q, d), 5.0, dtype=BF16, device=cuda)
+    got = ops.paged_prefill_attention(on(query, cuda), keys, values, table, offsets.to(cuda),
+                                      torch.tensor(starts).to(cuda), out=out, scale=scale)
+    assert ops.read_status(cuda) == 0
+    assert (got[:lead] == 5).all() and (got[rows - tail:] == 5).all()
+    scale = d ** -0.5 if scale is None else scale
+    for s, n in enumerate(counts):
+        for i in range(n):
+            r, seen = int(offsets[s]) + i, max(0, starts[s] + i + 1)
+            if n > 300 and i % 37 and i < n - 3:
+                continue
+            want, bound = attend(query[r], *case.sequence(s, seen), scale)
+            assert_within(got[r], want, bound, f"sequence {s} row {i} of {seen} keys")
+
+
+@pytest.mark.parametrize("q,kv,d", GEOMETRIES)
+def test_prompt_heads(ops, cuda, q, kv, d):
+    check_prompt(ops, cuda, q, kv, d, 32, [1, 33, 70, 5], [0, 0, 0, 0])
+
+
+@pytest.mark.parametrize("page", PAGES)
+@pytest.mark.parametrize("strided,one_pool", [(True, False), (False, True)])
+def test_prompt_pages_and_strides(ops, cuda, page, strided, one_pool):
+    check_prompt(ops, cuda, 16, 8, 128, page, [129, 1, 64, 200], [0, 31, 0, 5], strided=strided, one_pool=one_pool,
+                 columns=20)
+
+
+@pytest.mark.parametrize("counts,starts", [([1], [0]), ([127], [0]), ([128], [0]), ([129], [0]), ([257], [0]),
+                                           ([1, 1, 1], [0, 500, 129]), ([0, 5, 0, 0, 3, 0], [0, 0, 7, 0, 300, 0]),
+                                           ([40, 90], [1000, 64]), ([30, 6], [-7, -6]), ([3], [-5]), ([0], [0])])
+@pytest.mark.parametrize("q,kv,d", [(16, 8, 128), (8, 8, 64), (8, 1, 128)])
+def test_prompt_lengths_and_prefixes(ops, cuda, counts, starts, q, kv, d):
+    check_prompt(ops, cuda, q, kv, d, 64, counts, starts, lead=2, tail=3)
+
+
+def test_prompt_long(ops, cuda):
+    check_prompt(ops, cuda, 4, 1, 128, 64, [1500, 700], [0, 2000])
+    check_prompt(ops, cuda, 2, 2, 64, 16, [1500], [0], strided=True)
+
+
+def test_prompt_many_sequences(ops, cuda):
+    check_prompt(ops, cuda, 4, 2, 128, 16, [(13 * i) % 41 for i in range(120)], [(5 * i) % 23 for i in range(120)])
+
+
+def test_prompt_scale(ops, cuda):
+    check_prompt(ops, cuda, 16, 8, 128, 16, [150], [0], scale=0.5)
+    check_prompt(ops, cuda, 16, 8, 128, 16, [150], [0], scale=-0.25)
+
+
+def test_prompt_flags_bad_pages(ops, cuda):
+    case = Case([40, 40, 40], 8, 128, 16)
+    query = rows_of((120, 16, 128), 1, False)
+    keys, values, table = case.to(cuda)
+    offsets, starts = torch.tensor([0, 40, 80, 120], device=cuda), torch.zeros(3, dtype=torch.int64, device=cuda)
+
+    def prompt(page_table, start=starts):
+        got = ops.paged_prefill_attention(query.to(cuda), keys, values, page_table, offsets, start,
+                                          out=torch.zeros_like(query, device=cuda))
+        for r in list(range(40)) + list(range(80, 120)):
+            want, bound = attend(query[r], *case.sequence(r // 40, r % 40 + 1), 128 ** -0.5)
+            assert_within(got[r], want, bound, f"row {r}")
+        return ops.read_status(cuda)
+
+    assert prompt(table) == 0
+    for entry in (len(case.keys), -1, (1 << 31) - 1):
+        bad = table.clone()
+        bad[1, 1] = entry
+        assert prompt(bad) == 8
+    # a start that puts the rows past what the table can hold
+    assert prompt(table, torch.tensor([0, 20, 0], device=cuda)) == 8
+
+
+# ------------------------------------------------------------------ together
+def serve(ops, cuda, steps, capture):
+    """A prompt of three sequences, then `steps` decode steps, all through the pages; (outputs, their checks)."""
+    q, kv, d, page = 16, 8, 128, 16
+    counts = [37, 5, 64]
+    case = Case([n + steps for n in counts], kv, d, page, seed=4)
+    case.keys.fill_(float("nan")), case.values.fill_(float("nan"))
+    keys, values, table = case.to(cuda)
+    cos, sin = tables(128, d)
+    weights = [(1 + 0.2 * torch.randn(d, generator=rng(50 + i))).to(BF16) for i in range(2)]
+    dev = [t.to(cuda) for t in (*weights, cos, sin)]
+    rows = sum(counts)
+    qkv = torch.randn(rows + 3 * steps, (q + 2 * kv) * d, generator=rng(6)).to(BF16)
+    prompt, new = qkv[:rows].to(cuda), qkv[rows:].view(steps, 3, -1).to(cuda)
+    at = torch.cat([torch.arange(n) for n in counts]).to(cuda)
+    seq = torch.repeat_interleave(torch.arange(3), torch.tensor(counts)).to(cuda)
+    offsets = torch.tensor([0, 37, 42, 106], device=cuda)
+    heads = dict(q_heads=q, kv_heads=kv, head_dim=d)
+    queries = ops.paged_qk_norm_rope_kv(prompt, dev[0], dev[1], 1e-6, dev[2], dev[3], at, at, table, keys, values,
+                                        sequences=seq, **heads)
+    outs = [ops.paged_prefill_attention(queries, keys, values, table, offsets,
+                                        torch.zeros(3, dtype=torch.int64, device=cuda),
+                                        out=torch.empty_like(queries))]
+    positions, row = torch.tensor(counts, device=cuda), torch.empty_like(new[0])
+    out = torch.empty(3, q, d, dtype=BF16, device=cuda)
+
+    def step():
+        query = ops.paged_qk_norm_rope_kv(row, dev[0], dev[1], 1e-6, dev[2], dev[3], positions, positions, table, keys,
+                                          values, **heads)
+        ops.paged_decode_attention(query, keys, values, table, positions, out=out)
+        ops.advance(positions)
+
+    if capture:
+        row.copy_(new[0])
+        saved = positions.clone()
+        step()
+        positions.copy_(saved)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        positions.copy_(saved)
+    for i in range(steps):
+        row.copy_(new[i])
+        graph.replay() if capture else step()
+        outs.append(out.clone())
+    assert ops.read_status(cuda) == 0
+    return outs, (counts, qkv, weights, cos, sin)
+
+
+def check_served(outs, inputs, steps):
+    """Attention over the bf16 queries, keys and values of the write's own formula, in 64 bits. Where such a value lies
+    at a rounding boundary the kernel's may be one step off, so each score may move by 2^-7 of scale * sum |q k| twice."""
+    counts, qkv, weights, cos, sin = inputs
+    q, kv, d = 16, 8, 128
+    rows = sum(counts)
+    for s, n in enumerate(counts):
+        mine = torch.cat((qkv[sum(counts[:s]):sum(counts[:s]) + n], qkv[rows:].view(steps, 3, -1)[:, s]))
+        at = torch.arange(n + steps)
+        x = mine.view(-1, q + 2 * kv, d)
+        queries, keys = (turn(x[:, a:b], w, cos[at], sin[at], 1e-6)[0].to(BF16)
+                         for a, b, w in ((0, q, weights[0]), (q, q + kv, weights[1])))
+        values = x[:, q + kv:].double().transpose(0, 1)
+        for i in range(n + steps):
+            k, v = keys[:i + 1].double().transpose(0, 1), values[:, :i + 1]
+            want, bound = attend(queries[i], k, v, d ** -0.5)
+            got = outs[0][sum(counts[:s]) + i] if i < n else outs[1 + i - n][s]
+            # steps of a value at a boundary are rare: 1 element in 2^12 (fp32 error over a bf16 step), so at most a
+            # few of the 128 products of a score move, each by 2^-7 of itself
+            few = 4 * 2.0 ** -7 * d ** -0.5 * (queries[i].double().abs().amax() * k.abs().amax())
+            spread = v.abs().amax(1).repeat_interleave(2, 0)
+            assert_within(got, want, bound + 2 * few * spread, f"sequence {s} position {i}")
+
+
+@pytest.mark.parametrize("capture", [False, True])
+def test_serving_a_prompt_and_its_new_tokens(ops, cuda, capture):
+    outs, inputs = serve(ops, cuda, 20, capture)
+    check_served(outs, inputs, 20)
+
+
+def test_captured_and_eager_steps_agree_bit_for_bit(ops, cuda):
+    for a, b in zip(serve(ops, cuda, 6, False)[0], serve(ops, cuda, 6, True)[0]):
+        assert torch.equal(a, b)
+
+
+def test_two_graphs_and_an_eager_call_at_once(ops, cuda):
+    """Captured calls on two streams, replayed at the same time as eager ones on a third: nothing is shared."""
+    made = []
+    for i, lengths in enumerate(([9000, 20, 4000], [300] * 50, [12000])):
+        case = Case(lengths, 2, 128, 64, seed=i)
+        query = rows_of((len(lengths), 8, 128), 20 + i, False).to(cuda)
+        args = (query, *case.to(cuda), torch.tensor(lengths, device=cuda) - 1)
+        made.append((args, ops.paged_decode_attention(*args)))
+    graphs = []
+    for args, want in made[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.paged_decode_attention(*args)
+        graphs.append((graph, out, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for graph, out, _, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = ops.paged_decode_attention(*made[2][0])
+        torch.cuda.synchronize()
+        assert torch.equal(eager, made[2][1])
+        for _, out, want, _ in graphs:
+            assert torch.equal(out, want)
+            out.zero_()
+        torch.cuda.synchronize()
+
+
+def test_empty_batches_and_given_outputs(ops, cuda):
+    case = Case([20], 2, 64, 16)
+    keys, values, table = case.to(cuda)
+    none = torch.empty(0, dtype=torch.int64, device=cuda)
+    query = torch.empty(0, 4, 64, dtype=BF16, device=cuda)
+    assert ops.paged_decode_attention(query, keys, values, table[:0], none).shape == (0, 4, 64)
+    out = torch.empty_like(query)
+    assert ops.paged_prefill_attention(query, keys, values, table[:0], torch.zeros(1, dtype=torch.int64, device=cuda),
+                                       none, out=out) is out
+    cos, sin = (t.to(cuda) for t in tables(8, 64))
+    assert ops.paged_qk_norm_rope_kv(torch.empty(0, 8 * 64, dtype=BF16, device=cuda), None, None, 1e-6, cos, sin, none,
+                                     none, table, keys, values, q_heads=4, kv_heads=2, head_dim=64).shape == (0, 4, 64)
+    query = rows_of((1, 4, 64), 3, False).to(cuda)
+    out = torch.empty_like(query)
+    assert ops.paged_decode_attention(query, keys, values, table, torch.tensor([19], device=cuda), out=out) is out
+    assert_within(out[0], *attend(query[0].cpu(), *case.sequence(0, 20), 0.125))
