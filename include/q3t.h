@@ -387,41 +387,62 @@ int q3t_decode_attention_noalloc(const void* query, const void* keys, const void
  * are 16-byte aligned. What the pool holds at positions that no row sees does not matter, NaN included.
  */
 
+typedef struct {
+  const void* key_pages;
+  const void* value_pages;
+  int64_t page_stride, pages, page_size, kv_heads, head_dim;
+  const int32_t* page_table;
+  int64_t table_stride, table_rows, table_columns;
+  int64_t device; /* of every pointer and of the stream; negative: the current device */
+} q3t_paged_cache;
+
 /* Per-head q/k RMSNorm (norm weights nullable, both or none), rotate-half RoPE and the page write of
  * packed QKV rows: the paged form of q3t_qk_norm_rope_kv, with all arithmetic in fp32 and one
  * rounding to bf16. qkv: [rows, (q_heads + 2 kv_heads) * head_dim] (row stride qkv_stride, a multiple
  * of 8). Row r belongs to sequence sequences[r] (nullable: row r is sequence r, as in a decode step)
  * and writes its key and value at cache_positions[r]; cos/sin tables [table_len, head_dim] bf16 are
  * indexed by rotary_positions[r] (out of range: clamped, bad-index bit). A row with a negative
- * sequence is graph padding: nothing of it is read or written beyond that index. No two rows may
- * name the same position of a page. query_out: [rows, q_heads, head_dim]. */
-int q3t_paged_qk_norm_rope_kv(const void* qkv, int64_t qkv_stride, const void* q_norm_weight,
-                              const void* k_norm_weight, float eps, const void* cos_table,
-                              const void* sin_table, int64_t table_len, const int64_t* rotary_positions,
-                              const int64_t* cache_positions, const int64_t* sequences,
-                              const int32_t* page_table, int64_t table_stride, int64_t table_rows,
-                              int64_t table_columns, void* query_out, void* key_pages, void* value_pages,
-                              int64_t page_stride, int64_t pages, int64_t page_size, int64_t rows,
-                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, unsigned* status,
-                              void* stream);
+ * sequence is graph padding: it writes nothing and raises nothing. No two rows may name the same
+ * position of a page. query_out: [rows, q_heads, head_dim]. */
+typedef struct {
+  q3t_paged_cache cache;
+  const void* qkv;
+  int64_t qkv_stride, rows, q_heads;
+  const void* q_norm_weight;
+  const void* k_norm_weight;
+  const void* cos_table;
+  const void* sin_table;
+  int64_t table_len;
+  const int64_t* rotary_positions;
+  const int64_t* cache_positions;
+  const int64_t* sequences;
+  void* query_out;
+  double eps;
+} q3t_paged_write;
+int q3t_paged_qk_norm_rope_kv(const q3t_paged_write* call, unsigned* status, void* stream);
 
 /* Attention of one new token per sequence: query row r [q_heads, head_dim] (row stride query_stride, a
  * multiple of 8) sees keys 0 .. positions[r] of sequence r (page_table row r); positions[r] = -1 sees
- * none and gives zeros. positions < context <= columns * page_size (outside: clamped, bad-index bit);
- * a tighter context only helps the choice of the split. Any number of query heads per KV head.
- * out [rows, q_heads, head_dim], not overlapping query or pool. Results do not depend on the run: the
- * split over the keys and the order in which its parts are joined follow from positions and sizes.
+ * none and gives zeros. positions < context <= table_columns * page_size (outside: clamped, bad-index
+ * bit); a tighter context only helps the choice of the split. Any number of query heads per KV head.
+ * out [rows, q_heads, head_dim], not overlapping query or pool. Equal calls give equal bits: the split
+ * over the keys and the order in which its parts are joined follow from positions and sizes alone.
  * workspace: at least the queried size (0: NULL), 16-byte aligned, its contents of no matter before
  * and after; calls that may overlap on the GPU need one each. */
+typedef struct {
+  q3t_paged_cache cache;
+  const void* query;
+  int64_t query_stride, rows, q_heads;
+  const int64_t* positions;
+  void* out;
+  int64_t context;
+  double scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} q3t_paged_decode;
 size_t q3t_paged_decode_attention_workspace_bytes(int64_t rows, int64_t q_heads, int64_t kv_heads,
                                                   int64_t head_dim, int64_t context);
-int q3t_paged_decode_attention(const void* query, int64_t query_stride, const void* key_pages,
-                               const void* value_pages, int64_t page_stride, int64_t pages,
-                               int64_t page_size, const int32_t* page_table, int64_t table_stride,
-                               int64_t table_columns, const int64_t* positions, void* out, int64_t rows,
-                               int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t context,
-                               float scale, void* workspace, size_t workspace_bytes, unsigned* status,
-                               void* stream);
+int q3t_paged_decode_attention(const q3t_paged_decode* call, unsigned* status, void* stream);
 
 /* Causal attention of packed prompts over their pages. Sequence s owns query rows row_offsets[s] ..
  * row_offsets[s + 1] - 1 (int64 [sequences + 1], ascending, within 0 .. rows; sequences may be empty);
@@ -429,16 +450,21 @@ int q3t_paged_decode_attention(const void* query, int64_t query_stride, const vo
  * negative positions are left padding and give zeros) and sees keys 0 .. that position, all of which
  * the pool holds already and which are finite. Rows of no sequence are left as they are in out.
  * Otherwise as q3t_paged_decode_attention. */
+typedef struct {
+  q3t_paged_cache cache;
+  const void* query;
+  int64_t query_stride, rows, q_heads;
+  const int64_t* row_offsets;
+  const int64_t* start_positions;
+  int64_t sequences;
+  void* out;
+  double scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} q3t_paged_prefill;
 size_t q3t_paged_prefill_attention_workspace_bytes(int64_t rows, int64_t sequences, int64_t q_heads,
                                                    int64_t kv_heads, int64_t head_dim, int64_t context);
-int q3t_paged_prefill_attention(const void* query, int64_t query_stride, const void* key_pages,
-                                const void* value_pages, int64_t page_stride, int64_t pages,
-                                int64_t page_size, const int32_t* page_table, int64_t table_stride,
-                                int64_t table_columns, const int64_t* row_offsets,
-                                const int64_t* start_positions, int64_t sequences, void* out,
-                                int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
-                                float scale, void* workspace, size_t workspace_bytes, unsigned* status,
-                                void* stream);
+int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsigned* status, void* stream);
 
 /* ------------------------------------------------------------------ sampling */
 

@@ -69,20 +69,44 @@ int smem_limit(PerDevice& once, Kernel* kernel, int bytes, const char* what) {
       what);
 }
 
-// Checks of a paged key/value pool [pages, kv_heads, page_size, head_dim] (page stride in elements, everything
-// below it dense) and of the page table's shape; the same rules for every entry point that takes one.
-inline int check_pool(const char* name, int64_t page_stride, int64_t pages, int64_t page_size, int64_t kv_heads,
-                      int64_t head_dim, int64_t table_stride, int64_t table_rows, int64_t table_columns) {
-  if (pages < 1 || pages > 2147483647 || kv_heads < 1 || kv_heads > 1024)
+// Checks of a paged key/value pool (include/q3t.h) and of the page table's shape; the same rules for every entry
+// point that takes one.
+inline int check_cache(const char* name, const q3t_paged_cache& c) {
+  if (!c.key_pages || !c.value_pages || !c.page_table) return fail(Q3T_EINVAL, "%s: null pointer", name);
+  if (c.head_dim != 64 && c.head_dim != 128) return fail(Q3T_EUNSUPPORTED, "%s: head_dim must be 64 or 128", name);
+  if (c.pages < 1 || c.pages > 2147483647 || c.kv_heads < 1 || c.kv_heads > 1024)
     return fail(Q3T_EINVAL, "%s: invalid pool", name);
-  if (page_size < 16 || page_size > 65536 || page_size % 16)
+  if (c.page_size < 16 || c.page_size > 65536 || c.page_size % 16)
     return fail(Q3T_EUNSUPPORTED, "%s: page_size must be a multiple of 16 within 16..65536", name);
-  if (page_stride < kv_heads * page_size * head_dim || page_stride % 8 || page_stride > (int64_t(1) << 40))
+  if (c.page_stride < c.kv_heads * c.page_size * c.head_dim || c.page_stride % 8 ||
+      c.page_stride > (int64_t(1) << 36))
     return fail(Q3T_EINVAL, "%s: page stride", name);
-  if (table_rows < 1 || table_columns < 1 || table_columns > 2147483647 || (table_rows > 1 && table_stride < table_columns))
+  if (c.table_rows < 1 || c.table_columns < 1 || c.table_columns > 2147483647 ||
+      (c.table_rows > 1 && c.table_stride < c.table_columns))
     return fail(Q3T_EINVAL, "%s: invalid page table", name);
+  if (((reinterpret_cast<uintptr_t>(c.key_pages) | reinterpret_cast<uintptr_t>(c.value_pages)) & 15u) != 0)
+    return fail(Q3T_EINVAL, "%s: 16-byte alignment", name);
   return Q3T_OK;
 }
+
+// Makes `device` current for a call's launches and puts the caller's device back (negative: no change).
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(int64_t device) {
+    if (device < 0) return;
+    if (cudaGetDevice(&before_) != cudaSuccess) before_ = -1;
+    if (before_ == int(device)) before_ = -1;
+    else ok_ = before_ >= 0 && cudaSetDevice(int(device)) == cudaSuccess;
+  }
+  ~DeviceGuard() {
+    if (before_ >= 0) cudaSetDevice(before_);
+  }
+  bool ok() const { return ok_; }
+
+ private:
+  int before_ = -1;
+  bool ok_ = true;
+};
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 

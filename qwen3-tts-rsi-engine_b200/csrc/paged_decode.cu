@@ -337,37 +337,31 @@ int launch_direct(const DecodeArgs& a, const PromptRows& pr, void* stream, const
                 dim3(W * 32), size_t(C::kSmem), stream, true, name, a, pr);
 }
 
-int fill(DecodeArgs& a, const char* name, const void* query, int64_t query_stride, const void* key_pages,
-         const void* value_pages, int64_t page_stride, int64_t pages, int64_t page_size, const int32_t* page_table,
-         int64_t table_stride, int64_t table_rows, int64_t table_columns, void* out, int64_t rows, int64_t q_heads,
-         int64_t kv_heads, int64_t head_dim, float scale, unsigned* status) {
-  if (!query || !key_pages || !value_pages || !page_table || !out) return fail(Q3T_EINVAL, "%s: null pointer", name);
-  if (head_dim != 64 && head_dim != 128) return fail(Q3T_EUNSUPPORTED, "%s: head_dim must be 64 or 128", name);
-  if (const int rc = check_pool(name, page_stride, pages, page_size, kv_heads, head_dim, table_stride, table_rows,
-                                table_columns))
-    return rc;
-  if (rows < 1 || rows > (int64_t(1) << 30) || q_heads < 1 || q_heads > 1024 || q_heads % kv_heads)
+int fill(DecodeArgs& a, const char* name, const q3t_paged_cache& c, const void* query, int64_t query_stride,
+         int64_t rows, int64_t q_heads, void* out, double scale, unsigned* status) {
+  if (!query || !out) return fail(Q3T_EINVAL, "%s: null pointer", name);
+  if (const int rc = check_cache(name, c)) return rc;
+  if (rows < 1 || rows > (int64_t(1) << 30) || q_heads < 1 || q_heads > 1024 || q_heads % c.kv_heads)
     return fail(Q3T_EINVAL, "%s: invalid geometry", name);
-  if (query_stride < q_heads * head_dim || query_stride % 8) return fail(Q3T_EINVAL, "%s: query stride", name);
-  if (!aligned16(query) || !aligned16(key_pages) || !aligned16(value_pages) || !aligned16(out))
-    return fail(Q3T_EINVAL, "%s: 16-byte alignment", name);
+  if (query_stride < q_heads * c.head_dim || query_stride % 8) return fail(Q3T_EINVAL, "%s: query stride", name);
+  if (!aligned16(query) || !aligned16(out)) return fail(Q3T_EINVAL, "%s: 16-byte alignment", name);
   a.query = static_cast<const __nv_bfloat16*>(query);
-  a.keys = static_cast<const __nv_bfloat16*>(key_pages);
-  a.values = static_cast<const __nv_bfloat16*>(value_pages);
+  a.keys = static_cast<const __nv_bfloat16*>(c.key_pages);
+  a.values = static_cast<const __nv_bfloat16*>(c.value_pages);
   a.query_stride = query_stride;
-  a.page_stride = page_stride;
-  a.pages = PageTable{page_table, table_stride, table_rows, table_columns, pages, int(page_size)};
+  a.page_stride = c.page_stride;
+  a.pages = PageTable{c.page_table, c.table_stride, c.table_rows, c.table_columns, c.pages, int(c.page_size)};
   a.positions = nullptr;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.rows = int(rows);
   a.q_heads = int(q_heads);
-  a.kv_heads = int(kv_heads);
-  a.group = int(q_heads / kv_heads);
+  a.kv_heads = int(c.kv_heads);
+  a.group = int(q_heads / c.kv_heads);
   a.passes = (a.group + kHeads - 1) / kHeads;
-  a.context = table_columns * page_size;
-  a.scale_log2 = scale * kLog2e;
+  a.context = c.table_columns * c.page_size;
+  a.scale_log2 = float(scale) * kLog2e;
   a.status = status;
-  if (rows * kv_heads * a.passes > (int64_t(1) << 31) - 1) return fail(Q3T_EINVAL, "%s: too many rows", name);
+  if (rows * c.kv_heads * a.passes > (int64_t(1) << 31) - 1) return fail(Q3T_EINVAL, "%s: too many rows", name);
   return Q3T_OK;
 }
 
@@ -379,27 +373,22 @@ extern "C" size_t q3t_paged_decode_attention_workspace_bytes(int64_t rows, int64
   return 0;
 }
 
-extern "C" int q3t_paged_decode_attention(const void* query, int64_t query_stride, const void* key_pages,
-                                          const void* value_pages, int64_t page_stride, int64_t pages,
-                                          int64_t page_size, const int32_t* page_table, int64_t table_stride,
-                                          int64_t table_columns, const int64_t* positions, void* out, int64_t rows,
-                                          int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t context,
-                                          float scale, void* workspace, size_t workspace_bytes, unsigned* status,
-                                          void* stream) {
+extern "C" int q3t_paged_decode_attention(const q3t_paged_decode* call, unsigned* status, void* stream) {
   const char* name = "paged_decode_attention";
-  (void)workspace, (void)workspace_bytes;
+  if (call == nullptr) return fail(Q3T_EINVAL, "%s: null pointer", name);
+  const q3t_paged_decode& p = *call;
   DecodeArgs a;
-  if (const int rc = fill(a, name, query, query_stride, key_pages, value_pages, page_stride, pages, page_size,
-                          page_table, table_stride, rows, table_columns, out, rows, q_heads, kv_heads, head_dim, scale,
-                          status))
-    return rc;
-  if (!positions) return fail(Q3T_EINVAL, "%s: null pointer", name);
-  if (context < 1 || context > a.context) return fail(Q3T_EINVAL, "%s: context beyond the page table", name);
-  a.positions = positions;
-  a.context = context;
+  if (const int rc = fill(a, name, p.cache, p.query, p.query_stride, p.rows, p.q_heads, p.out, p.scale, status)) return rc;
+  if (!p.positions) return fail(Q3T_EINVAL, "%s: null pointer", name);
+  if (p.cache.table_rows < p.rows) return fail(Q3T_EINVAL, "%s: the page table needs a row per query row", name);
+  if (p.context < 1 || p.context > a.context) return fail(Q3T_EINVAL, "%s: context beyond the page table", name);
+  const DeviceGuard guard(p.cache.device);
+  if (!guard.ok()) return fail(Q3T_ECUDA, "%s: no such device", name);
+  a.positions = p.positions;
+  a.context = p.context;
   const PromptRows none = {};
-  return head_dim == 128 ? launch_direct<128, 8, 3, false>(a, none, stream, name)
-                         : launch_direct<64, 8, 6, false>(a, none, stream, name);
+  return p.cache.head_dim == 128 ? launch_direct<128, 8, 3, false>(a, none, stream, name)
+                                 : launch_direct<64, 8, 6, false>(a, none, stream, name);
 }
 
 extern "C" size_t q3t_paged_prefill_attention_workspace_bytes(int64_t rows, int64_t sequences, int64_t q_heads,
@@ -408,23 +397,18 @@ extern "C" size_t q3t_paged_prefill_attention_workspace_bytes(int64_t rows, int6
   return 0;
 }
 
-extern "C" int q3t_paged_prefill_attention(const void* query, int64_t query_stride, const void* key_pages,
-                                           const void* value_pages, int64_t page_stride, int64_t pages,
-                                           int64_t page_size, const int32_t* page_table, int64_t table_stride,
-                                           int64_t table_columns, const int64_t* row_offsets,
-                                           const int64_t* start_positions, int64_t sequences, void* out, int64_t rows,
-                                           int64_t q_heads, int64_t kv_heads, int64_t head_dim, float scale,
-                                           void* workspace, size_t workspace_bytes, unsigned* status, void* stream) {
+extern "C" int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsigned* status, void* stream) {
   const char* name = "paged_prefill_attention";
-  (void)workspace, (void)workspace_bytes;
+  if (call == nullptr) return fail(Q3T_EINVAL, "%s: null pointer", name);
+  const q3t_paged_prefill& p = *call;
   DecodeArgs a;
-  if (const int rc = fill(a, name, query, query_stride, key_pages, value_pages, page_stride, pages, page_size,
-                          page_table, table_stride, sequences, table_columns, out, rows, q_heads, kv_heads, head_dim,
-                          scale, status))
-    return rc;
-  if (!row_offsets || !start_positions) return fail(Q3T_EINVAL, "%s: null pointer", name);
-  if (sequences < 1 || sequences > (int64_t(1) << 20)) return fail(Q3T_EINVAL, "%s: invalid geometry", name);
-  const PromptRows pr = {row_offsets, start_positions, int(sequences)};
-  return head_dim == 128 ? launch_direct<128, 8, 3, true>(a, pr, stream, name)
-                         : launch_direct<64, 8, 6, true>(a, pr, stream, name);
+  if (const int rc = fill(a, name, p.cache, p.query, p.query_stride, p.rows, p.q_heads, p.out, p.scale, status)) return rc;
+  if (!p.row_offsets || !p.start_positions) return fail(Q3T_EINVAL, "%s: null pointer", name);
+  if (p.sequences < 1 || p.sequences > (int64_t(1) << 20) || p.cache.table_rows < p.sequences)
+    return fail(Q3T_EINVAL, "%s: invalid geometry", name);
+  const DeviceGuard guard(p.cache.device);
+  if (!guard.ok()) return fail(Q3T_ECUDA, "%s: no such device", name);
+  const PromptRows pr = {p.row_offsets, p.start_positions, int(p.sequences)};
+  return p.cache.head_dim == 128 ? launch_direct<128, 8, 3, true>(a, pr, stream, name)
+                                 : launch_direct<64, 8, 6, true>(a, pr, stream, name);
 }

@@ -119,54 +119,49 @@ __global__ void __launch_bounds__(kThreads) paged_write_kernel(const WriteArgs a
 
 }  // namespace
 
-extern "C" int q3t_paged_qk_norm_rope_kv(const void* qkv, int64_t qkv_stride, const void* q_norm_weight,
-                                         const void* k_norm_weight, float eps, const void* cos_table,
-                                         const void* sin_table, int64_t table_len, const int64_t* rotary_positions,
-                                         const int64_t* cache_positions, const int64_t* sequences,
-                                         const int32_t* page_table, int64_t table_stride, int64_t table_rows,
-                                         int64_t table_columns, void* query_out, void* key_pages, void* value_pages,
-                                         int64_t page_stride, int64_t pages, int64_t page_size, int64_t rows,
-                                         int64_t q_heads, int64_t kv_heads, int64_t head_dim, unsigned* status,
-                                         void* stream) {
+extern "C" int q3t_paged_qk_norm_rope_kv(const q3t_paged_write* call, unsigned* status, void* stream) {
   const char* name = "paged_qk_norm_rope_kv";
-  if (!qkv || !cos_table || !sin_table || !rotary_positions || !cache_positions || !page_table || !query_out ||
-      !key_pages || !value_pages || (q_norm_weight == nullptr) != (k_norm_weight == nullptr))
+  if (call == nullptr) return fail(Q3T_EINVAL, "%s: null pointer", name);
+  const q3t_paged_write& p = *call;
+  const q3t_paged_cache& c = p.cache;
+  if (!p.qkv || !p.cos_table || !p.sin_table || !p.rotary_positions || !p.cache_positions || !p.query_out ||
+      (p.q_norm_weight == nullptr) != (p.k_norm_weight == nullptr))
     return fail(Q3T_EINVAL, "%s: null pointer", name);
-  if (head_dim != 64 && head_dim != 128) return fail(Q3T_EUNSUPPORTED, "%s: head_dim must be 64 or 128", name);
-  if (const int rc = check_pool(name, page_stride, pages, page_size, kv_heads, head_dim, table_stride, table_rows,
-                                table_columns))
-    return rc;
-  if (rows < 1 || q_heads < 1 || q_heads > 1024 || table_len < 1 || (sequences == nullptr && table_rows < rows))
+  if (const int rc = check_cache(name, c)) return rc;
+  if (p.rows < 1 || p.q_heads < 1 || p.q_heads > 1024 || p.table_len < 1 ||
+      (p.sequences == nullptr && c.table_rows < p.rows))
     return fail(Q3T_EINVAL, "%s: invalid geometry", name);
-  const int64_t heads = q_heads + 2 * kv_heads;
-  if (qkv_stride < heads * head_dim || qkv_stride % 8) return fail(Q3T_EINVAL, "%s: qkv stride", name);
-  for (const void* p : {qkv, q_norm_weight, k_norm_weight, cos_table, sin_table, static_cast<const void*>(query_out),
-                        static_cast<const void*>(key_pages), static_cast<const void*>(value_pages)})
-    if (!aligned16(p)) return fail(Q3T_EINVAL, "%s: 16-byte alignment", name);
-  const int64_t per_block = kThreads / (head_dim / 8);
-  if (rows > (int64_t(1) << 31) / heads) return fail(Q3T_EINVAL, "%s: too many rows", name);
+  const int64_t heads = p.q_heads + 2 * c.kv_heads;
+  if (p.qkv_stride < heads * c.head_dim || p.qkv_stride % 8) return fail(Q3T_EINVAL, "%s: qkv stride", name);
+  if (!aligned16(p.qkv) || !aligned16(p.q_norm_weight) || !aligned16(p.k_norm_weight) || !aligned16(p.cos_table) ||
+      !aligned16(p.sin_table) || !aligned16(p.query_out))
+    return fail(Q3T_EINVAL, "%s: 16-byte alignment", name);
+  if (p.rows > (int64_t(1) << 31) / heads) return fail(Q3T_EINVAL, "%s: too many rows", name);
+  const DeviceGuard guard(c.device);
+  if (!guard.ok()) return fail(Q3T_ECUDA, "%s: no such device", name);
   WriteArgs a;
-  a.qkv = static_cast<const __nv_bfloat16*>(qkv);
-  a.qkv_stride = qkv_stride;
-  a.q_norm = static_cast<const __nv_bfloat16*>(q_norm_weight);
-  a.k_norm = static_cast<const __nv_bfloat16*>(k_norm_weight);
-  a.cos = static_cast<const __nv_bfloat16*>(cos_table);
-  a.sin = static_cast<const __nv_bfloat16*>(sin_table);
-  a.eps = eps;
-  a.table_len = table_len;
-  a.rotary_positions = rotary_positions;
-  a.cache_positions = cache_positions;
-  a.sequences = sequences;
-  a.pages = PageTable{page_table, table_stride, table_rows, table_columns, pages, int(page_size)};
-  a.query_out = static_cast<__nv_bfloat16*>(query_out);
-  a.key_pages = static_cast<__nv_bfloat16*>(key_pages);
-  a.value_pages = static_cast<__nv_bfloat16*>(value_pages);
-  a.page_stride = page_stride;
-  a.q_heads = int(q_heads);
-  a.kv_heads = int(kv_heads);
-  a.rows = rows;
+  a.qkv = static_cast<const __nv_bfloat16*>(p.qkv);
+  a.qkv_stride = p.qkv_stride;
+  a.q_norm = static_cast<const __nv_bfloat16*>(p.q_norm_weight);
+  a.k_norm = static_cast<const __nv_bfloat16*>(p.k_norm_weight);
+  a.cos = static_cast<const __nv_bfloat16*>(p.cos_table);
+  a.sin = static_cast<const __nv_bfloat16*>(p.sin_table);
+  a.eps = float(p.eps);
+  a.table_len = p.table_len;
+  a.rotary_positions = p.rotary_positions;
+  a.cache_positions = p.cache_positions;
+  a.sequences = p.sequences;
+  a.pages = PageTable{c.page_table, c.table_stride, c.table_rows, c.table_columns, c.pages, int(c.page_size)};
+  a.query_out = static_cast<__nv_bfloat16*>(p.query_out);
+  a.key_pages = static_cast<__nv_bfloat16*>(const_cast<void*>(c.key_pages));
+  a.value_pages = static_cast<__nv_bfloat16*>(const_cast<void*>(c.value_pages));
+  a.page_stride = c.page_stride;
+  a.q_heads = int(p.q_heads);
+  a.kv_heads = int(c.kv_heads);
+  a.rows = p.rows;
   a.status = status;
-  const dim3 grid(unsigned((rows * heads + per_block - 1) / per_block));
-  return launch(head_dim == 128 ? paged_write_kernel<128> : paged_write_kernel<64>, grid, dim3(kThreads), 0, stream,
+  const int64_t per_block = kThreads / (c.head_dim / 8);
+  const dim3 grid(unsigned((p.rows * heads + per_block - 1) / per_block));
+  return launch(c.head_dim == 128 ? paged_write_kernel<128> : paged_write_kernel<64>, grid, dim3(kThreads), 0, stream,
                 true, name, a);
 }

@@ -6,6 +6,7 @@ every operation raises - there is no CPU or library fallback behind these ops.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -36,6 +37,14 @@ class ChainStage(ctypes.Structure):
                 ("out_stride", ctypes.c_int64), ("out_dtype", ctypes.c_int), ("epilogue", ctypes.c_int),
                 ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64), ("bias", ctypes.c_void_p),
                 ("row_norm_eps", ctypes.c_float), ("depends", ctypes.c_int)]
+
+
+# Layouts of q3t_paged_write, q3t_paged_decode and q3t_paged_prefill (include/q3t.h): 8-byte fields only, packed by
+# one struct call because converting two dozen ctypes arguments costs as much as the launch itself (2 us).
+_PAGED_CACHE = "12q"
+PAGED_WRITE = struct.Struct(_PAGED_CACHE + "13qd")
+PAGED_DECODE = struct.Struct(_PAGED_CACHE + "7qd2q")
+PAGED_PREFILL = struct.Struct(_PAGED_CACHE + "8qd2q")
 
 
 # name -> (restype, argtypes); mirrors include/q3t.h exactly.
@@ -77,14 +86,11 @@ SIGNATURES: dict[str, tuple[object, list]] = {
                                             _i64, _f32, _p, _p]),
     "q3t_prefill_attention": (_i32, [_p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _p,
                                      _p]),
-    "q3t_paged_qk_norm_rope_kv": (_i32, [_p, _i64, _p, _p, _f32, _p, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p,
-                                         _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p]),
+    "q3t_paged_qk_norm_rope_kv": (_i32, [_p, _p, _p]),
     "q3t_paged_decode_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
-    "q3t_paged_decode_attention": (_i32, [_p, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64,
-                                          _i64, _i64, _i64, _f32, _p, _sz, _p, _p]),
+    "q3t_paged_decode_attention": (_i32, [_p, _p, _p]),
     "q3t_paged_prefill_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
-    "q3t_paged_prefill_attention": (_i32, [_p, _i64, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _p,
-                                           _i64, _i64, _i64, _i64, _f32, _p, _sz, _p, _p]),
+    "q3t_paged_prefill_attention": (_i32, [_p, _p, _p]),
     "q3t_cdf_select": (_i32, [_p, _p, _p, _i64, _i64, _p]),
     "q3t_sample": (_i32, [_p, _i32, _i64, _p, _i64, _p, _p, _i64, _i64, _f32, _f32, _i64, _f32, _p, _i64, _u64,
                           _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p]),

@@ -7,8 +7,8 @@ written, as the reference wrappers do.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 import math
 from typing import Optional
 
@@ -50,6 +50,7 @@ class Scratch:
     def __init__(self) -> None:
         self._buffers: dict[tuple, torch.Tensor] = {}
         self._status: dict[int, torch.Tensor] = {}
+        self._status_pointers: dict[int, int] = {}
 
     def workspace(self, nbytes: int, device: torch.device, tag: str = "default") -> torch.Tensor:
         key = (device.index if device.index is not None else torch.cuda.current_device(), tag)
@@ -71,6 +72,13 @@ class Scratch:
             word = torch.zeros(4, dtype=torch.int32, device=device)
             self._status[index] = word
         return word
+
+    def status_pointer(self, index: int) -> int:
+        """Address of the status word of device `index` (it lives as long as the process)."""
+        pointer = self._status_pointers.get(index)
+        if pointer is None:
+            pointer = self._status_pointers[index] = self.status(torch.device("cuda", index)).data_ptr()
+        return pointer
 
 
 SCRATCH = Scratch()
@@ -521,41 +529,65 @@ def decode_attention_qkv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin_
 
 
 # ------------------------------------------------------------------ paged key/value cache
-def _on(device: torch.device):
-    """The context in which to launch on `device`: the current one, or a switch to another GPU."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _check_paged(what: str, rows, key_pages, value_pages, page_table, **int64s) -> None:
-    """The checks that the paged operators share: `rows` is their bf16 input, int64s their index vectors."""
-    tensors = (rows, key_pages, value_pages, page_table, *int64s.values())
-    _need_cuda(*tensors)
-    device = rows.device
-    if any(t is not None and t.device != device for t in tensors):
-        raise ValueError(f"{what}: tensors must be on one device")
-    if (key_pages.ndim != 4 or key_pages.shape != value_pages.shape or key_pages.dtype != BF16
-            or value_pages.dtype != BF16 or rows.dtype != BF16):
-        raise ValueError(f"{what}: expected BF16 rows and BF16 key and value pages [pages, Hkv, page_size, D]")
-    _, _, size, dim = key_pages.shape
+# These wrappers are called once or twice per layer and token, so their checks read each attribute once and use the
+# cheap forms (get_device, identity of dtypes); the arguments travel as one packed struct.
+def _paged_cache(what: str, device: int, key_pages, value_pages, page_table):
+    """Check the pool and the page table; the leading fields of a packed call and the table's row count."""
+    if (device < 0 or key_pages.get_device() != device or value_pages.get_device() != device
+            or page_table.get_device() != device):
+        raise ValueError(f"{what}: expected CUDA tensors on one device")
+    if key_pages.dtype is not BF16 or value_pages.dtype is not BF16 or key_pages.dim() != 4:
+        raise ValueError(f"{what}: expected BF16 key and value pages [pages, Hkv, page_size, D]")
+    pages, heads, size, dim = shape = key_pages.shape
     stride = key_pages.stride()
-    if stride != value_pages.stride() or stride[1:] != (size * dim, dim, 1):
-        raise ValueError(f"{what}: pages must be dense [Hkv, page_size, D] blocks with one page stride")
-    if page_table.ndim != 2 or page_table.dtype != torch.int32 or page_table.stride(1) != 1:
-        raise ValueError(f"{what}: page table must be INT32 [sequences, columns] with unit inner stride")
-    for name, t in int64s.items():
-        if t is not None and (t.dtype != torch.int64 or t.ndim != 1 or not t.is_contiguous()):
-            raise ValueError(f"{what}: {name} must be a contiguous INT64 vector")
+    if (value_pages.shape != shape or value_pages.stride() != stride or stride[3] != 1 or stride[2] != dim
+            or stride[1] != size * dim):
+        raise ValueError(f"{what}: pages must be dense [Hkv, page_size, D] blocks, keys and values laid out alike")
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2:
+        raise ValueError(f"{what}: page table must be INT32 [sequences, columns]")
+    rows, columns = page_table.shape
+    row_stride, inner = page_table.stride()
+    if inner != 1:
+        raise ValueError(f"{what}: page table rows must have unit stride")
+    return (key_pages.data_ptr(), value_pages.data_ptr(), stride[0], pages, size, heads, dim, page_table.data_ptr(),
+            row_stride, rows, columns, device)
 
 
-def _check_query(what: str, query, key_pages, out) -> None:
-    if (query.ndim != 3 or query.shape[2] != key_pages.shape[3] or query.stride(2) != 1
-            or query.stride(1) != query.shape[2] or query.shape[1] % key_pages.shape[1]):
-        raise ValueError(f"{what}: query must be [rows, Hq, D] with dense rows, Hq a multiple of Hkv")
-    if out is not None and (out.shape != query.shape or out.dtype != BF16 or not out.is_contiguous()
-                            or out.device != query.device):
+def _paged_index(what: str, name: str, t, device: int, count: int) -> int:
+    if (t.get_device() != device or t.dtype is not torch.int64 or t.dim() != 1 or t.shape[0] != count
+            or not t.is_contiguous()):
+        raise ValueError(f"{what}: {name} must be a contiguous INT64 CUDA vector of {count}")
+    return t.data_ptr()
+
+
+def _paged_query(what: str, query, dim: int, kv_heads: int, out):
+    """(rows, query heads, row stride) of a query [rows, Hq, D] whose rows are dense."""
+    if query.dtype is not BF16 or query.dim() != 3:
+        raise ValueError(f"{what}: query must be BF16 [rows, Hq, D]")
+    rows, heads, width = shape = query.shape
+    stride = query.stride()
+    if width != dim or stride[2] != 1 or stride[1] != dim or heads % kv_heads:
+        raise ValueError(f"{what}: query rows must be dense [Hq, D], Hq a multiple of Hkv")
+    if out is not None and (out.shape != shape or out.dtype is not BF16 or not out.is_contiguous()
+                            or out.get_device() != query.get_device()):
         raise ValueError(f"{what}: out must be contiguous BF16 shaped like query")
+    return rows, heads, stride[0]
+
+
+def _paged_workspace(what: str, need: int, workspace, device: int):
+    """(tensor, pointer, bytes): the caller's workspace, or one of this call's own, from the caching allocator of
+    the current stream (inside a capture: of the graph). Calls and graphs never share one unasked."""
+    if workspace is None:
+        if need == 0:
+            return None, 0, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", device))
+    elif workspace.get_device() != device or not workspace.is_contiguous():
+        raise ValueError(f"{what}: workspace must be a contiguous tensor on the query's device")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _paged_call(name: str, packed: bytes, device: int) -> None:
+    call(name, packed, SCRATCH.status_pointer(device), torch._C._cuda_getCurrentRawStream(device))
 
 
 def paged_qk_norm_rope_kv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin_table, rotary_positions,
@@ -569,48 +601,45 @@ def paged_qk_norm_rope_kv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin
     sequence sequences[r] (None: of sequence r); rows with a negative sequence are skipped. No two rows may
     write the same position of a page. Returns the queries [rows, q_heads, head_dim]."""
     what = "paged_qk_norm_rope_kv"
-    _check_paged(what, qkv, key_pages, value_pages, page_table, rotary_positions=rotary_positions,
-                 cache_positions=cache_positions, sequences=sequences)
-    pages, heads, size, dim = key_pages.shape
-    if (qkv.ndim != 2 or qkv.stride(1) != 1 or heads != kv_heads or dim != head_dim
-            or qkv.shape[1] != (q_heads + 2 * kv_heads) * head_dim):
+    device = qkv.get_device()
+    cache = _paged_cache(what, device, key_pages, value_pages, page_table)
+    if qkv.dtype is not BF16 or qkv.dim() != 2 or cache[5] != kv_heads or cache[6] != head_dim:
+        raise ValueError(f"{what}: qkv must be BF16 [rows, (q + 2 kv) * head_dim] for the pages' heads")
+    rows, width = qkv.shape
+    row_stride, inner = qkv.stride()
+    if width != (q_heads + 2 * kv_heads) * head_dim or inner != 1:
         raise ValueError(f"{what}: qkv must be [rows, (q + 2 kv) * head_dim] with unit inner stride")
-    rows = qkv.shape[0]
-    if any(t is not None and t.shape[0] != rows for t in (rotary_positions, cache_positions, sequences)):
-        raise ValueError(f"{what}: positions and sequences must have one entry per row")
-    if sequences is None and page_table.shape[0] < rows:
+    rotary = _paged_index(what, "rotary_positions", rotary_positions, device, rows)
+    positions = _paged_index(what, "cache_positions", cache_positions, device, rows)
+    if sequences is not None:
+        sequences = _paged_index(what, "sequences", sequences, device, rows)
+    elif cache[9] < rows:
         raise ValueError(f"{what}: page table must have a row per qkv row")
-    for t, shape in ((q_norm_weight, (dim,)), (k_norm_weight, (dim,)), (cos_table, (cos_table.shape[0], dim)),
-                     (sin_table, (cos_table.shape[0], dim))):
-        if t is not None and (t.device != qkv.device or t.dtype != BF16 or t.shape != shape or not t.is_contiguous()):
-            raise ValueError(f"{what}: norm weights [head_dim] and cos/sin tables [positions, head_dim] must be "
-                             "contiguous BF16")
+    table_shape = cos_table.shape
+    if (cos_table.dtype is not BF16 or sin_table.dtype is not BF16 or cos_table.get_device() != device
+            or sin_table.get_device() != device or cos_table.dim() != 2 or table_shape[1] != head_dim
+            or sin_table.shape != table_shape or not cos_table.is_contiguous() or not sin_table.is_contiguous()):
+        raise ValueError(f"{what}: cos and sin tables must be contiguous BF16 [positions, head_dim]")
+    norms = 0, 0
+    if q_norm_weight is not None or k_norm_weight is not None:
+        for w in (q_norm_weight, k_norm_weight):
+            if (w is None or w.get_device() != device or w.dtype is not BF16 or w.numel() != head_dim
+                    or not w.is_contiguous()):
+                raise ValueError(f"{what}: norm weights must both be contiguous BF16 [head_dim], or both None")
+        norms = q_norm_weight.data_ptr(), k_norm_weight.data_ptr()
     if query_out is None:
-        query_out = torch.empty(rows, q_heads, dim, dtype=BF16, device=qkv.device)
-    elif (query_out.shape != (rows, q_heads, dim) or query_out.dtype != BF16 or not query_out.is_contiguous()
-          or query_out.device != qkv.device):
+        query_out = torch.empty(rows, q_heads, head_dim, dtype=BF16, device=qkv.device)
+    elif (query_out.get_device() != device or query_out.dtype is not BF16 or not query_out.is_contiguous()
+          or query_out.shape != (rows, q_heads, head_dim)):
         raise ValueError(f"{what}: query_out must be contiguous BF16 [rows, q_heads, head_dim]")
-    if rows == 0:
-        return query_out
-    with _on(qkv.device):
-        call("q3t_paged_qk_norm_rope_kv", qkv.data_ptr(), qkv.stride(0), _ptr(q_norm_weight), _ptr(k_norm_weight),
-             float(eps), cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0], rotary_positions.data_ptr(),
-             cache_positions.data_ptr(), _ptr(sequences), page_table.data_ptr(), page_table.stride(0),
-             page_table.shape[0], page_table.shape[1], query_out.data_ptr(), key_pages.data_ptr(),
-             value_pages.data_ptr(), key_pages.stride(0), pages, size, rows, q_heads, kv_heads, dim,
-             status_word(qkv.device).data_ptr(), _stream())
+    if rows:
+        _paged_call("q3t_paged_qk_norm_rope_kv", _lib.PAGED_WRITE.pack(
+            *cache, qkv.data_ptr(), row_stride, rows, q_heads, *norms, cos_table.data_ptr(), sin_table.data_ptr(),
+            table_shape[0], rotary, positions, sequences or 0, query_out.data_ptr(), eps), device)
     return query_out
 
 
-def _paged_workspace(what: str, need: int, workspace, device):
-    """The caller's workspace, or one of this call's own: calls and captured graphs never share it unasked."""
-    if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    if workspace.device != device or not workspace.is_contiguous():
-        raise ValueError(f"{what}: workspace must be a contiguous tensor on the query's device")
-    return workspace
-
-
+@functools.lru_cache(maxsize=1024)
 def paged_decode_attention_workspace_bytes(rows, q_heads, kv_heads, head_dim, context) -> int:
     return int(_lib.load().q3t_paged_decode_attention_workspace_bytes(rows, q_heads, kv_heads, head_dim, context))
 
@@ -624,28 +653,26 @@ def paged_decode_attention(query, key_pages, value_pages, page_table, positions,
     reaches (default: what the table can hold). `out` must not overlap query or pages. `workspace`: a buffer
     of paged_decode_attention_workspace_bytes that no other call uses meanwhile; by default the call takes its own."""
     what = "paged_decode_attention"
-    _check_paged(what, query, key_pages, value_pages, page_table, positions=positions)
-    _check_query(what, query, key_pages, out)
-    pages, kv_heads, size, dim = key_pages.shape
-    rows, q_heads, _ = query.shape
-    if positions.shape[0] != rows or page_table.shape[0] < rows:
-        raise ValueError(f"{what}: one position and a page table row per query row")
-    context = page_table.shape[1] * size if context is None else int(context)
-    scale = dim ** -0.5 if scale is None else float(scale)
-    out = torch.empty(query.shape, dtype=BF16, device=query.device) if out is None else out
-    if rows == 0:
-        return out
-    with _on(query.device):
-        ws = _paged_workspace(what, paged_decode_attention_workspace_bytes(rows, q_heads, kv_heads, dim, context),
-                              workspace, query.device)
-        call("q3t_paged_decode_attention", query.data_ptr(), query.stride(0), key_pages.data_ptr(),
-             value_pages.data_ptr(), key_pages.stride(0), pages, size, page_table.data_ptr(), page_table.stride(0),
-             page_table.shape[1], positions.data_ptr(), out.data_ptr(), rows, q_heads, kv_heads, dim, context, scale,
-             _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(), status_word(query.device).data_ptr(),
-             _stream())
+    device = query.get_device()
+    cache = _paged_cache(what, device, key_pages, value_pages, page_table)
+    _, _, _, _, size, kv_heads, dim, _, _, table_rows, columns, _ = cache
+    rows, q_heads, row_stride = _paged_query(what, query, dim, kv_heads, out)
+    at = _paged_index(what, "positions", positions, device, rows)
+    if table_rows < rows:
+        raise ValueError(f"{what}: page table must have a row per query row")
+    context = columns * size if context is None else int(context)
+    if out is None:
+        out = torch.empty(query.shape, dtype=BF16, device=query.device)
+    if rows:
+        need = paged_decode_attention_workspace_bytes(rows, q_heads, kv_heads, dim, context)
+        held, ws, ws_bytes = _paged_workspace(what, need, workspace, device)
+        _paged_call("q3t_paged_decode_attention", _lib.PAGED_DECODE.pack(
+            *cache, query.data_ptr(), row_stride, rows, q_heads, at, out.data_ptr(), context,
+            dim ** -0.5 if scale is None else scale, ws, ws_bytes), device)
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, head_dim, context) -> int:
     return int(_lib.load().q3t_paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, head_dim,
                                                                        context))
@@ -660,26 +687,21 @@ def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offse
     give zeros) and sees keys 0 .. that position in the pages of page_table[s], which hold them already. Rows
     that no sequence owns are left as they are in `out`. `workspace`: as for paged_decode_attention."""
     what = "paged_prefill_attention"
-    _check_paged(what, query, key_pages, value_pages, page_table, row_offsets=row_offsets,
-                 start_positions=start_positions)
-    _check_query(what, query, key_pages, out)
-    pages, kv_heads, size, dim = key_pages.shape
-    rows, q_heads, _ = query.shape
-    sequences = start_positions.shape[0]
-    if row_offsets.shape[0] != sequences + 1 or page_table.shape[0] < sequences:
-        raise ValueError(f"{what}: sequences + 1 row offsets and a page table row per start position")
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if rows == 0 or sequences == 0:
-        return out
-    with _on(query.device):
-        need = paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, dim,
-                                                       page_table.shape[1] * size)
-        ws = _paged_workspace(what, need, workspace, query.device)
-        call("q3t_paged_prefill_attention", query.data_ptr(), query.stride(0), key_pages.data_ptr(),
-             value_pages.data_ptr(), key_pages.stride(0), pages, size, page_table.data_ptr(), page_table.stride(0),
-             page_table.shape[1], row_offsets.data_ptr(), start_positions.data_ptr(), sequences, out.data_ptr(), rows,
-             q_heads, kv_heads, dim, scale, _ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(),
-             status_word(query.device).data_ptr(), _stream())
+    device = query.get_device()
+    cache = _paged_cache(what, device, key_pages, value_pages, page_table)
+    _, _, _, _, size, kv_heads, dim, _, _, table_rows, columns, _ = cache
+    rows, q_heads, row_stride = _paged_query(what, query, dim, kv_heads, out)
+    sequences = start_positions.numel()
+    starts = _paged_index(what, "start_positions", start_positions, device, sequences)
+    offsets = _paged_index(what, "row_offsets", row_offsets, device, sequences + 1)
+    if table_rows < sequences:
+        raise ValueError(f"{what}: page table must have a row per sequence")
+    if rows and sequences:
+        need = paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, dim, columns * size)
+        held, ws, ws_bytes = _paged_workspace(what, need, workspace, device)
+        _paged_call("q3t_paged_prefill_attention", _lib.PAGED_PREFILL.pack(
+            *cache, query.data_ptr(), row_stride, rows, q_heads, offsets, starts, sequences, out.data_ptr(),
+            dim ** -0.5 if scale is None else scale, ws, ws_bytes), device)
     return out
 
 

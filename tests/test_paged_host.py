@@ -92,6 +92,9 @@ class FakeCuda(torch.Tensor):
 
     device = property(lambda self: torch.device("cuda:0"))
 
+    def get_device(self):
+        return 0
+
     @classmethod
     def __torch_function__(cls, func, types, args=(), kwargs=None):
         out = super().__torch_function__(func, types, args, kwargs or {})
@@ -108,14 +111,11 @@ def no_launch(monkeypatch):
     class Reached(Exception):
         pass
 
-    def call(name, *args):
+    def call(name, packed, device):
         raise Reached(name)
 
-    monkeypatch.setattr(ops, "call", call)
-    monkeypatch.setattr(ops, "status_word", lambda device: torch.zeros(4, dtype=torch.int32))
-    monkeypatch.setattr(ops, "_stream", lambda: 0)
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
-    monkeypatch.setattr(ops, "_paged_workspace", lambda what, need, workspace, device: None)
+    monkeypatch.setattr(ops, "_paged_call", call)
+    monkeypatch.setattr(ops, "_paged_workspace", lambda what, need, workspace, device: (None, 0, 0))
     monkeypatch.setattr(ops, "paged_decode_attention_workspace_bytes", lambda *a: 0)
     monkeypatch.setattr(ops, "paged_prefill_attention_workspace_bytes", lambda *a: 0)
     return Reached
@@ -204,41 +204,40 @@ def test_cpu_tensors_are_refused():
 A16 = 1 << 20  # an aligned address that no call gets to use
 
 
+CACHE = dict(keys=A16, values=A16, page_stride=2048, pages=6, page_size=16, kv=2, dim=64, table=A16, table_stride=2,
+             table_rows=3, columns=2, device=-1)
+
+
+def c_call(name, layout, fields, change):
+    """A packed call with some fields changed, in the order of the C struct."""
+    assert set(change) <= {*CACHE, *fields}
+    values = [0 if v is None else v for v in ({**CACHE, **fields} | change).values()]
+    return getattr(_lib.load(), name)(layout.pack(*values), None, None)
+
+
 def c_decode(**change):
-    a = dict(query=A16, query_stride=256, keys=A16, values=A16, page_stride=2048, pages=6, page_size=16, table=A16,
-             table_stride=2, columns=2, positions=A16, out=A16, rows=3, q=4, kv=2, dim=64, context=32)
-    a.update(change)
-    return _lib.load().q3t_paged_decode_attention(
-        a["query"], a["query_stride"], a["keys"], a["values"], a["page_stride"], a["pages"], a["page_size"], a["table"],
-        a["table_stride"], a["columns"], a["positions"], a["out"], a["rows"], a["q"], a["kv"], a["dim"], a["context"],
-        0.125, None, 0, None, None)
+    return c_call("q3t_paged_decode_attention", _lib.PAGED_DECODE, dict(
+        query=A16, query_stride=256, rows=3, q=4, positions=A16, out=A16, context=32, scale=0.125, workspace=None,
+        workspace_bytes=0), change)
 
 
 def c_prompt(**change):
-    a = dict(query=A16, query_stride=256, keys=A16, values=A16, page_stride=2048, pages=6, page_size=16, table=A16,
-             table_stride=2, columns=2, offsets=A16, starts=A16, sequences=3, out=A16, rows=9, q=4, kv=2, dim=64)
-    a.update(change)
-    return _lib.load().q3t_paged_prefill_attention(
-        a["query"], a["query_stride"], a["keys"], a["values"], a["page_stride"], a["pages"], a["page_size"], a["table"],
-        a["table_stride"], a["columns"], a["offsets"], a["starts"], a["sequences"], a["out"], a["rows"], a["q"], a["kv"],
-        a["dim"], 0.125, None, 0, None, None)
+    return c_call("q3t_paged_prefill_attention", _lib.PAGED_PREFILL, dict(
+        query=A16, query_stride=256, rows=9, q=4, offsets=A16, starts=A16, sequences=3, out=A16, scale=0.125,
+        workspace=None, workspace_bytes=0), change)
 
 
 def c_write(**change):
-    a = dict(qkv=A16, stride=512, qw=A16, kw=A16, cos=A16, sin=A16, length=9, rotary=A16, at=A16, sequences=None, table=A16,
-             table_stride=2, table_rows=3, columns=2, query=A16, keys=A16, values=A16, page_stride=2048, pages=6,
-             page_size=16, rows=3, q=4, kv=2, dim=64)
-    a.update(change)
-    return _lib.load().q3t_paged_qk_norm_rope_kv(
-        a["qkv"], a["stride"], a["qw"], a["kw"], 1e-6, a["cos"], a["sin"], a["length"], a["rotary"], a["at"],
-        a["sequences"], a["table"], a["table_stride"], a["table_rows"], a["columns"], a["query"], a["keys"], a["values"],
-        a["page_stride"], a["pages"], a["page_size"], a["rows"], a["q"], a["kv"], a["dim"], None, None)
+    return c_call("q3t_paged_qk_norm_rope_kv", _lib.PAGED_WRITE, dict(
+        qkv=A16, stride=512, rows=3, q=4, qw=A16, kw=A16, cos=A16, sin=A16, length=9, rotary=A16, at=A16,
+        sequences=None, query=A16, eps=1e-6), change)
 
 
 POOLS = [(dict(keys=None), -1), (dict(values=A16 + 2), -1), (dict(page_stride=2047), -1), (dict(page_stride=1 << 41), -1),
          (dict(pages=0), -1), (dict(pages=1 << 31), -1), (dict(page_size=24), -2), (dict(page_size=0), -2),
          (dict(page_size=1 << 20), -2), (dict(kv=0), -1), (dict(dim=96), -2), (dict(table=None), -1),
-         (dict(columns=0), -1), (dict(table_stride=1), -1), (dict(rows=0), -1)]
+         (dict(columns=0), -1), (dict(table_stride=1), -1), (dict(rows=0), -1),
+         (dict(table_rows=0), -1), (dict(table_rows=2), -1)]
 C_BAD = [(c_decode, c, rc) for c, rc in POOLS + [
     (dict(query_stride=255), -1), (dict(query_stride=260), -1), (dict(q=5), -1), (dict(query=A16 + 8), -1),
     (dict(context=33), -1), (dict(context=0), -1), (dict(positions=None), -1), (dict(rows=1 << 31), -1)]]
@@ -246,7 +245,28 @@ C_BAD += [(c_prompt, c, rc) for c, rc in POOLS + [
     (dict(offsets=None), -1), (dict(starts=None), -1), (dict(sequences=0), -1), (dict(out=A16 + 4), -1), (dict(q=3), -1)]]
 C_BAD += [(c_write, c, rc) for c, rc in POOLS + [
     (dict(stride=511), -1), (dict(stride=516), -1), (dict(qw=None), -1), (dict(cos=None), -1), (dict(length=0), -1),
-    (dict(qkv=A16 + 8), -1), (dict(table_rows=2), -1), (dict(rows=1 << 40), -1)]]
+    (dict(qkv=A16 + 8), -1), (dict(rows=1 << 40), -1)]]
+
+
+def test_packed_layouts_match_the_header(tmp_path):
+    """sizeof the C structs, and the offset of the last field of each, as a C compiler sees them."""
+    compiler = shutil.which("gcc")
+    if compiler is None:
+        pytest.skip("gcc not found")
+    source = tmp_path / "sizes.c"
+    source.write_text("""#include <stdio.h>
+#include "q3t.h"
+int main(void) {
+  printf("%zu %zu %zu %zu %zu %zu %zu\\n", sizeof(q3t_paged_cache), sizeof(q3t_paged_write), sizeof(q3t_paged_decode),
+         sizeof(q3t_paged_prefill), offsetof(q3t_paged_write, eps), offsetof(q3t_paged_decode, scale),
+         offsetof(q3t_paged_prefill, scale));
+  return 0;
+}
+""")
+    subprocess.run([compiler, "-std=c99", "-I", str(ROOT / "include"), str(source), "-o", str(tmp_path / "sizes")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True).stdout.split()]
+    sizes = [s.size for s in (_lib.PAGED_WRITE, _lib.PAGED_DECODE, _lib.PAGED_PREFILL)]
+    assert got == [96, *sizes, sizes[0] - 8, sizes[1] - 24, sizes[2] - 24]
 
 
 @pytest.mark.parametrize("entry,change,rc", C_BAD, ids=lambda v: getattr(v, "__name__", None) or str(v))
