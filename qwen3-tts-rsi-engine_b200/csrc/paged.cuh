@@ -37,6 +37,8 @@ constexpr int kStepKeys = 16;
 // Steps of a row at `position` (the row sees keys 0 .. position; -1: none).
 Q3T_HD int64_t steps_of(int64_t position) { return position < 0 ? 0 : position / kStepKeys + 1; }
 
+// The ranges that `total` steps are split into where at most `parts` can work: none of them is empty.
+Q3T_HD int64_t split_parts(int64_t total, int64_t parts) { return total < parts ? total : parts; }
 // `total` steps in `parts` even contiguous ranges: part i holds [split_begin(i), split_begin(i + 1)).
 // total * parts stays below 2^63: a pool holds fewer than 2^47 steps and parts are at most 2^14.
 Q3T_HD int64_t split_begin(int64_t i, int64_t total, int64_t parts) { return i * total / parts; }

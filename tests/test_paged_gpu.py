@@ -132,31 +132,46 @@ def check_decode(ops, cuda, q, kv, d, page, lengths, *, strided=False, one_pool=
         assert_within(got[r], want, bound, f"row {r} of {n} keys")
 
 
+# The table's capacity is all that a call knows of the lengths beforehand: one that could hold very long contexts
+# makes it cut the keys of all rows into even ranges instead of going row by row.
+BOTH = pytest.mark.parametrize("capacity", [None, 1 << 17], ids=["rows", "ranges"])
+
+
+def columns_for(capacity, page):
+    return None if capacity is None else capacity // page
+
+
+@BOTH
 @pytest.mark.parametrize("q,kv,d", GEOMETRIES)
-def test_decode_heads(ops, cuda, q, kv, d):
-    check_decode(ops, cuda, q, kv, d, 32, [1, 0, 15, 16, 17, 31, 32, 33, 127, 128, 129, 400])
+def test_decode_heads(ops, cuda, q, kv, d, capacity):
+    check_decode(ops, cuda, q, kv, d, 32, [1, 0, 15, 16, 17, 31, 32, 33, 127, 128, 129, 400],
+                 columns=columns_for(capacity, 32))
 
 
+@BOTH
 @pytest.mark.parametrize("page", PAGES)
 @pytest.mark.parametrize("strided,one_pool", [(True, False), (False, True)])
-def test_decode_pages_and_strides(ops, cuda, page, strided, one_pool):
+def test_decode_pages_and_strides(ops, cuda, page, strided, one_pool, capacity):
     check_decode(ops, cuda, 16, 8, 128, page, [page - 1, page, page + 1, 5 * page + 3], strided=strided,
-                 one_pool=one_pool, columns=9)
+                 one_pool=one_pool, columns=columns_for(capacity, page) or 9)
 
 
 @pytest.mark.parametrize("lengths", [[1], [0], [0, 0, 0], [4097], [1, 8000, 1], [3000] + [5] * 40, [513] * 70])
 @pytest.mark.parametrize("q,kv,d", [(16, 8, 128), (16, 1, 64)])
-def test_decode_lengths(ops, cuda, lengths, q, kv, d):
-    check_decode(ops, cuda, q, kv, d, 64, lengths)
+@BOTH
+def test_decode_lengths(ops, cuda, lengths, q, kv, d, capacity):
+    check_decode(ops, cuda, q, kv, d, 64, lengths, columns=columns_for(capacity, 64))
 
 
 def test_decode_long_context(ops, cuda):
     check_decode(ops, cuda, 8, 2, 128, 128, [70001, 1, 33333])
 
 
-@pytest.mark.parametrize("count", [300, 1500])
-def test_decode_many_rows(ops, cuda, count):
-    check_decode(ops, cuda, 4, 2, 64, 16, [(37 * i) % 90 for i in range(count)], seed=count)
+@BOTH
+@pytest.mark.parametrize("count", [30, 300, 1500, 4097])
+def test_decode_many_rows(ops, cuda, count, capacity):
+    check_decode(ops, cuda, 4, 2, 64, 16, [(37 * i) % 90 for i in range(count)], seed=count,
+                 columns=columns_for(capacity, 16))
 
 
 def test_decode_context_bound_shared_pages_and_scale(ops, cuda):
@@ -166,10 +181,11 @@ def test_decode_context_bound_shared_pages_and_scale(ops, cuda):
     check_decode(ops, cuda, 16, 8, 128, 16, [90, 41, 64, 3], scale=0.0)
 
 
-def test_decode_rising_scores_move_the_reference(ops, cuda):
+@BOTH
+def test_decode_rising_scores_move_the_reference(ops, cuda, capacity):
     """Scores that grow by far more than the lazy margin from step to step, up and down again."""
     n, d = 300, 64
-    case = Case([n], 1, d, 16)
+    case = Case([n], 1, d, 16, columns=columns_for(capacity, 16))
     keys, _ = case.sequence(0, n)
     ramp = torch.cat((torch.arange(200.0), torch.arange(100.0).flip(0)))
     for j in range(n):
@@ -182,11 +198,12 @@ def test_decode_rising_scores_move_the_reference(ops, cuda):
     assert_within(got[0], want, bound)
 
 
-def test_decode_infinite_scores_follow_the_formula(ops, cuda):
+@BOTH
+def test_decode_infinite_scores_follow_the_formula(ops, cuda, capacity):
     """A key of -inf has weight 0 wherever it stands; only -inf scores, or one of +inf, have no value."""
     n, d = 40, 64
     for where in (0, 5, 39):
-        case = Case([n], 1, d, 16)
+        case = Case([n], 1, d, 16, columns=columns_for(capacity, 16))
         case.keys[case.table[0, where // 16], 0, where % 16, 0] = -float("inf")
         query = torch.ones(1, 1, d, dtype=BF16)
         k, v, table = case.to(cuda)
@@ -203,10 +220,11 @@ def test_decode_infinite_scores_follow_the_formula(ops, cuda):
     assert got.isnan().all()
 
 
-def test_decode_flags_bad_positions_and_pages(ops, cuda):
+@BOTH
+def test_decode_flags_bad_positions_and_pages(ops, cuda, capacity):
     """The row with the bad index is unspecified; its neighbours are right and nothing faults."""
     lengths = [40, 40, 40]
-    case = Case(lengths, 8, 128, 16)
+    case = Case(lengths, 8, 128, 16, columns=columns_for(capacity, 16))
     query = rows_of((3, 16, 128), 1, False)
     keys, values, table = case.to(cuda)
 
@@ -226,17 +244,18 @@ def test_decode_flags_bad_positions_and_pages(ops, cuda):
 
 
 def test_decode_clamps_a_position_past_the_context(ops, cuda):
-    case = Case([64, 64], 8, 128, 16)
+    case = Case([64, 64], 8, 128, 16, columns=9)
     query = rows_of((2, 16, 128), 1, False)
     keys, values, table = case.to(cuda)
-    got = ops.paged_decode_attention(query.to(cuda), keys, values, table, torch.tensor([64, 20], device=cuda))
+    got = ops.paged_decode_attention(query.to(cuda), keys, values, table, torch.tensor([64, 20], device=cuda), context=64)
     assert ops.read_status(cuda) == 8
     assert_within(got[0], *attend(query[0], *case.sequence(0, 64), 128 ** -0.5))
     assert_within(got[1], *attend(query[1], *case.sequence(1, 21), 128 ** -0.5))
 
 
-def test_decode_repeats_bit_for_bit(ops, cuda):
-    case = Case([5000, 77, 1234, 1], 8, 128, 64)
+@BOTH
+def test_decode_repeats_bit_for_bit(ops, cuda, capacity):
+    case = Case([5000, 77, 1234, 1], 8, 128, 64, columns=columns_for(capacity, 64))
     query = rows_of((4, 16, 128), 1, False).to(cuda)
     keys, values, table = case.to(cuda)
     at = torch.tensor([4999, 76, 1233, 0], device=cuda)
@@ -414,7 +433,7 @@ def test_two_graphs_and_an_eager_call_at_once(ops, cuda):
     """Captured calls on two streams, replayed at the same time as eager ones on a third: nothing is shared."""
     made = []
     for i, lengths in enumerate(([9000, 20, 4000], [300] * 50, [12000])):
-        case = Case(lengths, 2, 128, 64, seed=i)
+        case = Case(lengths, 2, 128, 64, seed=i, columns=2048)
         query = rows_of((len(lengths), 8, 128), 20 + i, False).to(cuda)
         args = (query, *case.to(cuda), torch.tensor(lengths, device=cuda) - 1)
         made.append((args, ops.paged_decode_attention(*args)))
@@ -436,6 +455,25 @@ def test_two_graphs_and_an_eager_call_at_once(ops, cuda):
             assert torch.equal(out, want)
             out.zero_()
         torch.cuda.synchronize()
+
+
+def test_a_workspace_of_the_caller(ops, cuda):
+    """Where a call needs one: the queried size is enough, whatever it holds; a smaller one is refused."""
+    case = Case([700, 3], 8, 128, 64, columns=2048)
+    query = rows_of((2, 16, 128), 1, False).to(cuda)
+    keys, values, table = case.to(cuda)
+    at = torch.tensor([699, 2], device=cuda)
+    want = ops.paged_decode_attention(query, keys, values, table, at)
+    need = ops.paged_decode_attention_workspace_bytes(2, 16, 8, 128, 2048 * 64)
+    assert need > 0
+    held = torch.full((need + 64,), 255, dtype=torch.uint8, device=cuda)
+    got = ops.paged_decode_attention(query, keys, values, table, at, workspace=held[:need])
+    assert torch.equal(got, want) and held[need:].eq(255).all()
+    for bad in (held[:need - 16], held[8:]):
+        with pytest.raises(ValueError, match="workspace"):
+            ops.paged_decode_attention(query, keys, values, table, at, workspace=bad)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.paged_decode_attention(query, keys, values, table, at, workspace=held.cpu())
 
 
 def test_empty_batches_and_given_outputs(ops, cuda):

@@ -38,6 +38,9 @@ int main() {
   // even splits: the ranges tile [0, total), differ by one at most, and split_owner inverts them
   for (int64_t total : {1, 2, 7, 8, 9, 147, 148, 149, 1000, 4097})
     for (int64_t parts : {1, 2, 8, 148, 296, 1184}) {
+      const int64_t ranges = split_parts(total, parts);
+      for (int64_t i = 0; i < ranges; ++i) CHECK(split_begin(i + 1, total, ranges) > split_begin(i, total, ranges));
+      CHECK(ranges <= parts && split_parts(0, parts) == 0);
       CHECK(split_begin(0, total, parts) == 0 && split_begin(parts, total, parts) == total);
       for (int64_t i = 0; i < parts; ++i) {
         const int64_t b = split_begin(i, total, parts), e = split_begin(i + 1, total, parts);
