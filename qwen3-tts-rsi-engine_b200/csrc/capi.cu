@@ -88,6 +88,24 @@ int make_map_bf16_3d(CUtensorMap* map, const void* base, int64_t d0, int64_t d1,
   return Q3T_OK;
 }
 
+int make_map_bf16_strided(CUtensorMap* map, const void* base, const int64_t (&dims)[4], const int64_t (&strides)[3],
+                          const int (&box)[4], int rank) {
+  EncodeTiled enc = tiled_encoder();
+  if (enc == nullptr) return fail(Q3T_ECUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t d[4], st[3];
+  cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = cuuint64_t(dims[i]);
+    b[i] = cuuint32_t(box[i]);
+    if (i + 1 < rank) st[i] = cuuint64_t(strides[i]) * 2;
+  }
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(rank), const_cast<void*>(base), d, st, b, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(Q3T_EINVAL, "tensor map encode failed (%d)", int(r));
+  return Q3T_OK;
+}
+
 }  // namespace q3t
 
 extern "C" int q3t_abi_version(void) { return 1; }

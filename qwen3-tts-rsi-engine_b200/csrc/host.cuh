@@ -32,6 +32,10 @@ int make_map_bf16(CUtensorMap* map, const void* base, int64_t rows, int64_t cols
 int make_map_bf16_3d(CUtensorMap* map, const void* base, int64_t d0, int64_t d1, int64_t d2, int box0, int box1,
                      int box2);
 
+// `rank`-D (2..4) bf16 tensor map with the strides of dims 1.. in elements, 128-byte swizzle.
+int make_map_bf16_strided(CUtensorMap* map, const void* base, const int64_t (&dims)[4], const int64_t (&strides)[3],
+                          const int (&box)[4], int rank);
+
 // A per-device one-time set-up (a kernel attribute, a cached query): `run(init)`
 // calls init() for the current device until it first succeeds, under a mutex, so
 // host threads that make their first calls concurrently neither race on the flag

@@ -26,6 +26,7 @@
 #include "common.cuh"
 #include "host.cuh"
 #include "paged.cuh"
+#include "paged_prefill.cuh"
 
 using namespace q3t;
 
@@ -844,6 +845,7 @@ extern "C" int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsign
     return fail(Q3T_EINVAL, "%s: invalid geometry", name);
   const DeviceGuard guard(p.cache.device);
   if (!guard.ok()) return fail(Q3T_ECUDA, "%s: no such device", name);
+  if (prefill_tiles_supported(p)) return launch_prefill_tiles(p, status, stream, name);
   const PromptRows pr = {p.row_offsets, p.start_positions, int(p.sequences)};
   return p.cache.head_dim == 128 ? launch_direct<128, 8, 2, true>(a, pr, 1, stream, name)
                                  : launch_direct<64, 8, 4, true>(a, pr, 1, stream, name);

@@ -1,0 +1,12 @@
+// The tensor-core form of q3t_paged_prefill_attention (paged_prefill.cu); arguments are checked by the caller.
+#pragma once
+
+#include "q3t.h"
+
+namespace q3t {
+
+// Whether sizes and scale are within what the tiled kernel takes (its counters are 32-bit, its scale positive).
+bool prefill_tiles_supported(const q3t_paged_prefill& call);
+int launch_prefill_tiles(const q3t_paged_prefill& call, unsigned* status, void* stream, const char* name);
+
+}  // namespace q3t
