@@ -112,6 +112,33 @@ Q3T_DEV float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Two fp32 operations in one instruction.
+Q3T_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+Q3T_DEV float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+Q3T_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Moves registers between the warpgroups: the CTA is launched with kThreads * 168, and 56 + 2 * 224 = 3 * 168.
+constexpr int kRegsLoad = 56, kRegsSoftmax = 224;
+static_assert(kRegsLoad + 2 * kRegsSoftmax == 3 * 168, "register shares must add up to the launch's");
 Q3T_DEV uint32_t pack2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
@@ -227,6 +254,100 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
 
+  if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    // ---------------- softmax: thread = query row = TMEM lane
+    const int t = (warp >> 2) - 1, m = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t s_at = lanes + 128 * t, o_at = lanes + 256 + 128 * t;
+    const int p = m / a.heads, h = m % a.heads;
+    const bool real = p < count[t] && unit % a.passes * a.heads + h < a.group;
+    const int64_t position = tile.position + t * a.positions + p;
+    const int last = int(position < -1 ? -1 : position < a.capacity ? position : a.capacity - 1);  // last key seen
+    float top = -INFINITY, sum = 0.f;
+    bool ok = true;
+    for (int j = 0; j < tiles[t]; ++j) {
+      if (!warp_wait(&bars->s_full[t], j, a.status, kStatusMmaTimeout)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float s[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, s + 32 * c);
+      tmem_ld_wait();
+      const int seen = last + 1 - j * kTileKeys;  // keys of this tile that the row sees
+      if (__any_sync(0xffffffffu, seen < kTileKeys)) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < 128; i += 2) mx[i / 2 & 3] = max3(mx[i / 2 & 3], s[i], s[i + 1]);
+      const float now = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+      if (__any_sync(0xffffffffu, now > top + 8.f || (top == -INFINITY && now > top))) {
+        const float to = fmaxf(top, now);
+        const float f = to == top ? 1.f : exp2_fast(top - to);
+        top = to;
+        sum *= f;
+        if (j > 0) {  // the products up to tile j - 1 are done: s_full says so
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tmem_ld32(o_at + 32 * c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= f;
+            tmem_st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
+          }
+        }
+      }
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
+      float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float2 x = fma2(make_float2(s[64 * c + 2 * i], s[64 * c + 2 * i + 1]), scale2, ref2);
+          x.x = exp2_fast(x.x);
+          x.y = exp2_fast(x.y);
+          part[i & 1] = add2(part[i & 1], x);
+          w[i] = pack2(x.x, x.y);
+        }
+        tmem_st32(s_at + 32 * c, w);
+      }
+      sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&bars->p_full[t]);
+    }
+    // ---- O / l
+    if (tiles[t] > 0) ok = ok && warp_wait(&bars->o_done[t], 0, a.status, kStatusMmaTimeout);
+    tc_fence_after();
+    __nv_bfloat16* to = a.out + (int64_t(tile.row + t * a.positions + p) * a.q_heads + head0 + h) * D;
+    const float inv = last < 0 ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      float o[32];
+      if (tiles[t] > 0 && ok) {  // uniform over the warp
+        tmem_ld32(o_at + 32 * c, o);
+        tmem_ld_wait();
+      }
+      if (real && ok) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = last < 0 ? 0.f : o[8 * i + e] * inv;
+          *reinterpret_cast<uint4*>(to + 32 * c + 8 * i) = pack8(v);
+        }
+      }
+    }
+    tc_fence_before();
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
   if (warp == 0) {
     // ---------------- loads
     bool ok = true;
@@ -342,96 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(&bars->done);
       mbar_wait(&bars->done, 0, a.status, kStatusMmaTimeout);
     }
-  } else if (warp >= 4) {
-    // ---------------- softmax: thread = query row = TMEM lane
-    const int t = (warp >> 2) - 1, m = (warp & 3) * 32 + lane;
-    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t s_at = lanes + 128 * t, o_at = lanes + 256 + 128 * t;
-    const int p = m / a.heads, h = m % a.heads;
-    const bool real = p < count[t] && unit % a.passes * a.heads + h < a.group;
-    const int64_t position = tile.position + t * a.positions + p;
-    const int last = int(position < -1 ? -1 : position < a.capacity ? position : a.capacity - 1);  // last key seen
-    float top = -INFINITY, sum = 0.f;
-    bool ok = true;
-    for (int j = 0; j < tiles[t]; ++j) {
-      if (!warp_wait(&bars->s_full[t], j, a.status, kStatusMmaTimeout)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      float s[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, s + 32 * c);
-      tmem_ld_wait();
-      const int seen = last + 1 - j * kTileKeys;  // keys of this tile that the row sees
-      if (__any_sync(0xffffffffu, seen < kTileKeys)) {
-#pragma unroll
-        for (int i = 0; i < 128; ++i) s[i] = i < seen ? s[i] : -INFINITY;
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-      const float now = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-      if (__any_sync(0xffffffffu, now > top + 8.f || (top == -INFINITY && now > top))) {
-        const float to = fmaxf(top, now);
-        const float f = to == top ? 1.f : exp2_fast(top - to);
-        top = to;
-        sum *= f;
-        if (j > 0) {  // the products up to tile j - 1 are done: s_full says so
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            tmem_ld32(o_at + 32 * c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= f;
-            tmem_st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
-          }
-        }
-      }
-      const float ref = top == -INFINITY ? 0.f : top;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float x = exp2_fast(fmaf(s[64 * c + 2 * i], a.scale_log2, -ref));
-          const float y = exp2_fast(fmaf(s[64 * c + 2 * i + 1], a.scale_log2, -ref));
-          part[2 * (i & 1)] += x;
-          part[2 * (i & 1) + 1] += y;
-          w[i] = pack2(x, y);
-        }
-        tmem_st32(s_at + 32 * c, w);
-      }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&bars->p_full[t]);
-    }
-    // ---- O / l
-    if (tiles[t] > 0) ok = ok && warp_wait(&bars->o_done[t], 0, a.status, kStatusMmaTimeout);
-    tc_fence_after();
-    __nv_bfloat16* to = a.out + (int64_t(tile.row + t * a.positions + p) * a.q_heads + head0 + h) * D;
-    const float inv = last < 0 ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      float o[32];
-      if (tiles[t] > 0 && ok) {  // uniform over the warp
-        tmem_ld32(o_at + 32 * c, o);
-        tmem_ld_wait();
-      }
-      if (real && ok) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = last < 0 ? 0.f : o[8 * i + e] * inv;
-          *reinterpret_cast<uint4*>(to + 32 * c + 8 * i) = pack8(v);
-        }
-      }
-    }
-    tc_fence_before();
+  }
   }
   __syncthreads();
   if (warp == 2) {
