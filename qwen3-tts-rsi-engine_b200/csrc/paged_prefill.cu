@@ -63,24 +63,46 @@ Q3T_DEV void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem]: A bf16, two values of a row per 32-bit column.
-Q3T_DEV void umma_bf16_ta(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The issuing warp stays converged and computes every operand warp-uniformly (tcgen05.mma takes them from uniform
+// registers); `leader` is set in one lane, which alone issues. With the addresses computed by a single lane instead,
+// moving them over took longer than the products (100 cycles an instruction of 64).
+Q3T_DEV bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(e));
+  return e != 0;
+}
+// Descriptor words: start address, leading stride | stride 1024, version 1, 128-byte swizzle (see umma_desc_sw128).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+Q3T_DEV uint64_t desc_of(uint32_t lo) { return (uint64_t(kDescHi) << 32) | lo; }
+// K-major operand at `addr`; its next 16 columns are 2 further on.
+Q3T_DEV uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+// MN-major operand: 64 columns x 8 rows per 1024-byte atom, the next 64 columns `block` bytes on; the next 16 rows
+// are 128 further on.
+Q3T_DEV uint32_t desc_mn(uint32_t addr, uint32_t block) { return (addr >> 4) | ((block >> 4) << 16); }
+// D[tmem] (+)= A[smem] * B[smem]
+Q3T_DEV void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, bool add, bool leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(desc_of(a_lo)), "l"(desc_of(b_lo)), "r"(idesc), "r"(uint32_t(add)), "r"(uint32_t(leader))
       : "memory");
 }
-// MN-major SW128 operand: 64 columns x 8 rows per 1024-byte atom, the next 64 columns `block` bytes on.
-Q3T_DEV uint64_t desc_mn(uint32_t addr, uint32_t block) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>((block >> 4) & 0x3FFFu) << 16;
-  d |= static_cast<uint64_t>(1024u >> 4) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  d |= static_cast<uint64_t>(2u) << 61;
-  return d;
+// D[tmem] (+)= A[tmem] * B[smem]: A bf16, two values of a row per 32-bit column.
+Q3T_DEV void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, bool add, bool leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(desc_of(b_lo)), "r"(idesc), "r"(uint32_t(add)), "r"(uint32_t(leader))
+      : "memory");
+}
+Q3T_DEV void commit_if(uint64_t* bar, bool leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(uint32_t(leader))
+      : "memory");
 }
 Q3T_DEV void tmem_ld32(uint32_t addr, float* v) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -400,27 +422,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(i & 1 ? &bars->v_full[(i / 2) % kStages] : &bars->k_full[(i / 2) % kStages], (i / 2 / kStages) & 1, a.status,
                   kStatusTmaTimeout);
   } else if (warp == 1) {
-    // ---------------- products
+    // ---------------- products (TMEM column 0 is the allocation's first: it is all of TMEM)
     constexpr uint32_t idesc_s = umma_idesc_bf16(128, kTileKeys);
     constexpr uint32_t idesc_o = umma_idesc_bf16(128, D) | (1u << 16);  // V MN-major
+    const uint32_t base = smem_u32(smem);
+    const bool leader = elect_one();
     bool ok = true;
-    auto scores = [&](int t, int s) {
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-        umma_bf16(tmem + 128 * t, umma_desc_sw128(smem_u32(smem + t * M::kTile + (k >> 2) * M::kBlock)) + 2 * (k & 3),
-                  umma_desc_sw128(smem_u32(smem + M::kK + s * M::kTile + (k >> 2) * M::kBlock)) + 2 * (k & 3), idesc_s, k > 0);
-      umma_commit(&bars->s_full[t]);
-    };
     auto wait = [&](uint64_t* bar, int phase, unsigned bit) { ok = ok && warp_wait(bar, phase, a.status, bit); };
+    auto scores = [&](int t, int s) {
+      const uint32_t q = desc_k(base + t * M::kTile), k = desc_k(base + M::kK + s * M::kTile);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t step = (i >> 2) * (M::kBlock >> 4) + 2 * (i & 3);
+        mma_ss(128 * t, q + step, k + step, idesc_s, i > 0, leader);
+      }
+      commit_if(&bars->s_full[t], leader);
+    };
     if (key_tiles > 0) {
       wait(&bars->k_full[0], 0, kStatusTmaTimeout);
       for (int t = 0; t < 2; ++t) {
         if (tiles[t] == 0) continue;
         wait(&bars->q_full[t], 0, kStatusTmaTimeout);
         tc_fence_after();
-        if (ok && lane == 0) scores(t, 0);
+        if (ok) scores(t, 0);
       }
-      if (ok && lane == 0) umma_commit(&bars->k_empty[0]);
+      if (ok) commit_if(&bars->k_empty[0], leader);
     }
     for (int j = 0; j < key_tiles && ok; ++j) {
       const int s = j % kStages, phase = j / kStages, sn = (j + 1) % kStages;
@@ -435,28 +461,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_async_shared();
         __syncwarp();
       }
-      bool next_ready = false;
+      if (j + 1 < key_tiles) wait(&bars->k_full[sn], (j + 1) / kStages, kStatusTmaTimeout);
+      const uint32_t v = desc_mn(base + M::kV + s * M::kTile, M::kBlock);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (j >= tiles[t]) continue;
         wait(&bars->p_full[t], j, kStatusMmaTimeout);
         tc_fence_after();
-        if (ok && lane == 0) {
+        if (!ok) continue;
 #pragma unroll
-          for (int k = 0; k < kTileKeys / 16; ++k)
-            umma_bf16_ta(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k,
-                         desc_mn(smem_u32(smem + M::kV + s * M::kTile + k * 16 * 128), M::kBlock), idesc_o, j > 0 || k > 0);
-          if (j + 1 >= tiles[t]) umma_commit(&bars->o_done[t]);
-        }
-        if (j + 1 < tiles[t]) {
-          if (!next_ready) wait(&bars->k_full[sn], (j + 1) / kStages, kStatusTmaTimeout);
-          next_ready = true;
-          if (ok && lane == 0) scores(t, sn);
-        }
+        for (int i = 0; i < kTileKeys / 16; ++i)
+          mma_ts(256 + 128 * t, 128 * t + 8 * i, v + 128 * i, idesc_o, j > 0 || i > 0, leader);
+        if (j + 1 < tiles[t]) scores(t, sn);
+        else commit_if(&bars->o_done[t], leader);
       }
-      if (ok && lane == 0) {
-        umma_commit(&bars->v_empty[s]);
-        if (j + 1 < key_tiles) umma_commit(&bars->k_empty[sn]);
+      if (ok) {
+        commit_if(&bars->v_empty[s], leader);
+        if (j + 1 < key_tiles) commit_if(&bars->k_empty[sn], leader);
       }
     }
     if (lane == 0) {  // every product is done before TMEM is released
