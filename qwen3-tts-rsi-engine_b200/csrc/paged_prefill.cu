@@ -50,8 +50,7 @@ struct Smem {
 };
 
 struct Bars {
-  uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2],
-      o_done[2], done;
+  uint64_t q_full[2], k_full[kStages], v_full[kStages], turn[2], s_full[2], p_full[2][2], o_done[2], done;
   uint32_t tmem;
 };
 
@@ -240,14 +239,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars->q_full[i], 1);
         mbar_init(&bars->s_full[i], 1);
-        mbar_init(&bars->p_full[i], 128);
+        mbar_init(&bars->turn[i], 1);
+        mbar_init(&bars->p_full[i][0], 128);
+        mbar_init(&bars->p_full[i][1], 128);
         mbar_init(&bars->o_done[i], 1);
       }
       for (int i = 0; i < kStages; ++i) {
         mbar_init(&bars->k_full[i], 1);
-        mbar_init(&bars->k_empty[i], 1);
         mbar_init(&bars->v_full[i], 1);
-        mbar_init(&bars->v_empty[i], 1);
       }
       mbar_init(&bars->done, 1);
       fence_mbar_init();
@@ -339,11 +338,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           w[i] = pack2(x.x, x.y);
         }
         tmem_st32(s_at + 32 * c, w);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full[t][c]);
       }
       sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&bars->p_full[t]);
     }
     // ---- O / l
     if (tiles[t] > 0) ok = ok && warp_wait(&bars->o_done[t], 0, a.status, kStatusMmaTimeout);
@@ -402,12 +401,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int wanted = min(pieces, (keys - j * kTileKeys + a.piece - 1) / a.piece);  // pieces that hold a key
       const uint32_t bytes = uint32_t(wanted * a.piece * 128 * kHalves);
 #pragma unroll
-      for (int v = 0; v < 2; ++v) {
+      for (int v = 0; v < 2 && ok; ++v) {
+        // turn i of the products has read key tile i and value tile i - 1
+        const int turn = j - kStages + v;
+        if (j >= kStages) ok = warp_wait(&bars->turn[turn & 1], turn >> 1, a.status, kStatusMmaTimeout);
+        if (!ok) break;
         uint64_t* full = v ? &bars->v_full[s] : &bars->k_full[s];
-        if (j >= kStages && !warp_wait(v ? &bars->v_empty[s] : &bars->k_empty[s], j / kStages - 1, a.status, kStatusMmaTimeout)) {
-          ok = false;
-          break;
-        }
         if (lane == 0) mbar_expect_tx(full, bytes);
         __syncwarp();
         if (piece < wanted)
@@ -446,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         if (ok) scores(t, 0);
       }
-      if (ok) commit_if(&bars->k_empty[0], leader);
+      if (ok) commit_if(&bars->turn[0], leader);
     }
     for (int j = 0; j < key_tiles && ok; ++j) {
       const int s = j % kStages, phase = j / kStages, sn = (j + 1) % kStages;
@@ -466,19 +465,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (j >= tiles[t]) continue;
-        wait(&bars->p_full[t], j, kStatusMmaTimeout);
-        tc_fence_after();
-        if (!ok) continue;
 #pragma unroll
-        for (int i = 0; i < kTileKeys / 16; ++i)
-          mma_ts(256 + 128 * t, 128 * t + 8 * i, v + 128 * i, idesc_o, j > 0 || i > 0, leader);
+        for (int half = 0; half < 2; ++half) {  // the first 64 keys' weights come before the others are computed
+          wait(&bars->p_full[t][half], j, kStatusMmaTimeout);
+          tc_fence_after();
+          if (!ok) continue;
+#pragma unroll
+          for (int i = 4 * half; i < 4 * half + 4; ++i)
+            mma_ts(256 + 128 * t, 128 * t + 8 * i, v + 128 * i, idesc_o, j > 0 || i > 0, leader);
+        }
+        if (!ok) continue;
         if (j + 1 < tiles[t]) scores(t, sn);
         else commit_if(&bars->o_done[t], leader);
       }
-      if (ok) {
-        commit_if(&bars->v_empty[s], leader);
-        if (j + 1 < key_tiles) commit_if(&bars->k_empty[sn], leader);
-      }
+      if (ok) commit_if(&bars->turn[(j + 1) & 1], leader);
     }
     if (lane == 0) {  // every product is done before TMEM is released
       umma_commit(&bars->done);
