@@ -830,8 +830,8 @@ extern "C" int q3t_paged_decode_attention(const q3t_paged_decode* call, unsigned
 
 extern "C" size_t q3t_paged_prefill_attention_workspace_bytes(int64_t rows, int64_t sequences, int64_t q_heads,
                                                               int64_t kv_heads, int64_t head_dim, int64_t context) {
-  (void)rows, (void)sequences, (void)q_heads, (void)kv_heads, (void)head_dim, (void)context;
-  return 0;
+  if (rows < 1 || sequences < 1 || q_heads < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
+  return prefill_tiles_workspace(rows, sequences, q_heads, kv_heads, head_dim, context);
 }
 
 extern "C" int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsigned* status, void* stream) {

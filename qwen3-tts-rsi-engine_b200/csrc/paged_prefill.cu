@@ -10,10 +10,18 @@
 //   P_t = 2^(S_t scale log2e - m)   one thread per query row; bf16, over S_t's own TMEM columns
 //   O_t += P_t V       tcgen05.mma 128 x D x 128, P from TMEM, V as the MN-major operand
 //
-// Warps 4-7 and 8-11 are the softmax of tile 0 and 1, warp 0 loads, warp 1 issues the products: while one tile's
-// weights are computed the tensor cores run the other's products. m is a reference that the row's maximum exceeds by at
-// most 8 (powers of two), so O in TMEM is rescaled only when a maximum moves by more; O / l does not depend on it.
-// P's rounding to bf16 is that of a bf16 tensor product; S, m, l and O stay in fp32.
+// Warps 4-7 and 8-11 are the softmax of tile 0 and 1, warp 0 loads, warp 1 issues the products, warp 3 hands out the
+// work: while one tile's weights are computed the tensor cores run the other's products. m is a reference that the
+// row's maximum exceeds by at most 8 (powers of two), so O in TMEM is rescaled only when a maximum moves by more; O / l
+// does not depend on it. P's rounding to bf16 is that of a bf16 tensor product; S, m, l and O stay in fp32.
+//
+// Work comes in one of two ways (the host picks by sizes):
+// - items (query tile pair, KV head) in turn: a CTA whose item's loads are out takes over one that has not been launched
+//   yet, so items go to the SMs as those get free, and the next one's loads and first products overlap the last one's
+//   softmax and stores (16 prompts of 256 rows: 22.4 us against 23.9 with a CTA each);
+// - one even range of all items' key tiles per CTA, one CTA per SM. An item that a range covers only in part leaves O, m
+//   and l in the workspace, and a second, dependent launch joins the parts in the order of their keys (results repeat
+//   bit for bit). Parts are never smaller than kLeast tiles: short items move to one range whole.
 #include "common.cuh"
 #include "host.cuh"
 #include "paged.cuh"
@@ -27,6 +35,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileKeys = 128, kTileRows = 128;
 constexpr int kStages = 2;  // of K, and of V
 constexpr int kThreads = 384;
+constexpr int kLeast = 4;          // key tiles of a part
+constexpr int kFixed = 2;          // what an item costs beside its key tiles, in key tiles
+constexpr int kPlanTiles = 2048;   // query tile pairs and sequences that a range plan holds
+constexpr int kPlanSequences = 1024;
 
 struct PrefillArgs {
   PageTable pages;
@@ -37,22 +49,45 @@ struct PrefillArgs {
   int passes, positions;  // passes over the group; positions of a tile
   int piece;    // rows of a TMA box: gcd(page_size, 128)
   int capacity; // positions that a page table row can hold
+  bool out_32;  // out is 32-byte aligned
+  int items;    // at most
+  int parts;    // ranges, one per CTA; 0: whole items in turn
+  struct Segment* shared_segments;  // workspace: [parts][2], what a range left unfinished at its start (0) and end (1)
+  float* partial;                   // workspace: [parts][2][D / 4][256 rows][4], then [256][2] (m, l)
   float scale_log2;
   unsigned* status;
+};
+
+// A run of key tiles of one item.
+struct Segment {
+  int sequence, row, count;            // the tile pair's first packed row and rows (positions); count 0: no more work
+  int head, head0, heads;              // KV head; first query head and query heads of the pass
+  int tile0, key_tiles, all_tiles;     // key tiles of the run, and of the item
+  int slot;                            // -1: the whole item; else where the run's O, m and l wait for the join
+  int64_t position;                    // of the first row
 };
 
 template <int D>
 struct Smem {
   static constexpr int kTile = 128 * D * 2;  // a query, key or value tile: D / 64 blocks of 128 rows x 128 bytes
   static constexpr int kBlock = 128 * 128;
-  static constexpr int kK = 2 * kTile, kV = kK + kStages * kTile, kBar = kV + kStages * kTile;
-  static constexpr int kBytes = kBar + 256 + 1024;
+  static constexpr int kK = 2 * kTile, kV = kK + kStages * kTile, kPlan = kV + kStages * kTile;
+  static constexpr int kBar = kPlan + (kPlanTiles + 1 + kPlanSequences + 1) * 4 + 8;
+  static constexpr int kBytes = (kBar + 15) / 16 * 16 + 512 + 1024;
 };
 
 struct Bars {
-  uint64_t q_full[2], k_full[kStages], v_full[kStages], turn[2], s_full[2], p_full[2][2], o_done[2], done;
+  uint64_t q_full[2], q_free[2], k_full[kStages], v_full[kStages], turn[2], s_full[2], p_full[2][2], o_done[2], o_free[2],
+      segment_full[2], segment_free[2], loaded, takeover, done;
+  alignas(16) uint4 response;
+  Segment segments[2];
+  int sums[kThreads / 32];
   uint32_t tmem;
 };
+
+// floats of a part in the workspace
+template <int D>
+constexpr int kPartFloats = 256 * (D + 2);
 
 // One 4-D tiled load; x * 2 bytes is a multiple of 16 (0 or 64 elements).
 Q3T_DEV void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
@@ -115,18 +150,26 @@ Q3T_DEV void tmem_ld32(uint32_t addr, float* v) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
-Q3T_DEV void tmem_st32(uint32_t addr, const uint32_t* r) {
+Q3T_DEV void tmem_st16(uint32_t addr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
       : "memory");
 }
-Q3T_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for tcgen05.ld; the 32 registers pass through, so that nothing reads (or moves) them before. With more than 32,
+// the others pass through an empty statement behind the wait.
+template <bool WAIT = true>
+Q3T_DEV void tmem_ld_wait(float* v) {
+  if constexpr (WAIT) asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  asm volatile(""
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                 "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+                 "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+                 "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
 Q3T_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 Q3T_DEV float exp2_fast(float x) {
   float y;
@@ -157,6 +200,23 @@ Q3T_DEV float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// 2^x of two values without the special-function unit, whose 16 results a cycle and SM the kernel is short of:
+// x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low bits), then 2^f on [-1/2, 1/2] as
+// 1 + a polynomial of degree 4 (fitted here for the least maximal relative error: 2^-18.4) and n added to the exponent.
+// From x = -127 down the result is exactly 0: f is 0 there, and 1.0's exponent becomes 0. Not for NaN.
+Q3T_DEV float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
+  const float2 n = add2(x, make_float2(12582912.f, 12582912.f));
+  const float2 f = add2(x, fma2(n, make_float2(-1.f, -1.f), make_float2(12582912.f, 12582912.f)));
+  float2 p = fma2(make_float2(0.009585323743522167f, 0.009585323743522167f), f,
+                  make_float2(0.05590662732720375f, 0.05590662732720375f));
+  p = fma2(p, f, make_float2(0.24024039506912231f, 0.24024039506912231f));
+  p = fma2(p, f, make_float2(0.6931241750717163f, 0.6931241750717163f));
+  p = fma2(p, f, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
+}
 // Moves registers between the warpgroups: the CTA is launched with kThreads * 168, and 56 + 2 * 224 = 3 * 168.
 constexpr int kRegsLoad = 56, kRegsSoftmax = 224;
 static_assert(kRegsLoad + 2 * kRegsSoftmax == 3 * 168, "register shares must add up to the launch's");
@@ -165,34 +225,72 @@ Q3T_DEV uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// Asks for a CTA of this grid that has not been launched yet; the answer comes through `bar`. After a refusal it is not
+// asked again.
+Q3T_DEV void try_take_over(uint4* response, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(response)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+Q3T_DEV bool taken_over(const uint4* response, int& block) {
+  uint32_t yes, x;
+  ulonglong2 r;
+  asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(r.x), "=l"(r.y) : "r"(smem_u32(response)) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tmov.b128 r, {%2, %3};\n\tmov.u32 %1, 0;\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}\n"
+      : "=r"(yes), "=r"(x)
+      : "l"(r.x), "l"(r.y));
+  block = int(x);
+  return yes != 0;
+}
+// 32 bytes to memory, in one store where the address allows it.
+Q3T_DEV void store32(void* to, const uint32_t* w, bool aligned) {
+  if (aligned) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(to)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(to)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
 // A bounded wait of a whole warp: every lane leaves with the same answer.
 Q3T_DEV bool warp_wait(uint64_t* bar, int phase, unsigned* status, unsigned bits) {
   return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, status, bits));
 }
 
-// What a CTA works on. Work items are numbered from the last tile of the last sequence backwards, so that
-// the tiles with the most keys start first.
-struct Tile {
-  int sequence, row, count;  // first packed row and rows (positions)
-  int64_t position;          // of the first row
-};
+// The packed rows of sequence s and the first of them; 0 where the offsets make no sense.
+Q3T_DEV int rows_of(const PrefillArgs& a, int s, int& first) {
+  const int64_t lo = a.row_offsets[s], hi = a.row_offsets[s + 1];
+  if (lo >= 0 && hi <= a.rows && hi > lo) {
+    first = int(lo);
+    return int(hi - lo);
+  }
+  if (hi != lo) raise_status(a.status, kStatusBadIndex);
+  first = 0;
+  return 0;
+}
+// Keys that rows up to position `end` - 1 see (what the table cannot hold is cut off), and their tiles.
+Q3T_DEV int keys_of(const PrefillArgs& a, int64_t end) { return end < 0 ? 0 : int(end < a.capacity ? end : a.capacity); }
+Q3T_DEV int key_tiles_of(const PrefillArgs& a, int64_t end) { return (keys_of(a, end) + kTileKeys - 1) / kTileKeys; }
 
-// Found by one warp; count 0: no such tile.
-Q3T_DEV Tile find_tile(const PrefillArgs& a, int index, int lane) {
+// Query tile pairs are numbered from the last of the last sequence backwards, so that those with the most keys
+// come first. One warp finds the sequence, rows and key tiles of number `index`; count 0: there is none.
+Q3T_DEV Segment find_tile(const PrefillArgs& a, int index, int unit, int lane) {
   const int span = 2 * a.positions;
+  Segment t = {};
   for (int base = a.sequences - 1; base >= 0; base -= 32) {
     const int s = base - lane;
     int n = 0, first = 0, tiles = 0;
+    int64_t start = 0;
     if (s >= 0) {
-      const int64_t lo = a.row_offsets[s], hi = a.row_offsets[s + 1];
-      if (lo >= 0 && hi <= a.rows && hi > lo) {
-        first = int(lo);
-        n = int(hi - lo);
-        tiles = (n + span - 1) / span;
-      } else if (hi != lo) {
-        raise_status(a.status, kStatusBadIndex);
-      }
+      start = a.start_positions[s];
+      n = rows_of(a, s, first);
     }
+    tiles = (n + span - 1) / span;
     int sum = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -205,16 +303,58 @@ Q3T_DEV Tile find_tile(const PrefillArgs& a, int index, int lane) {
       continue;
     }
     const int src = __ffs(hit) - 1;
-    Tile t;
-    const int tile = (tiles - 1) - (index - (sum - tiles));  // counted from the sequence's last tile
-    t.sequence = __shfl_sync(0xffffffffu, s, src);
-    t.row = __shfl_sync(0xffffffffu, first + tile * span, src);
-    t.count = __shfl_sync(0xffffffffu, min(span, n - tile * span), src);
-    const int in_sequence = __shfl_sync(0xffffffffu, tile * span, src);
-    t.position = a.start_positions[t.sequence] + in_sequence;
-    return t;
+    const int in_sequence = ((tiles - 1) - (index - (sum - tiles))) * span;  // counted from the sequence's last tile
+    t.sequence = base - src;
+    t.row = __shfl_sync(0xffffffffu, first + in_sequence, src);
+    t.count = __shfl_sync(0xffffffffu, min(span, n - in_sequence), src);
+    t.position = __shfl_sync(0xffffffffu, start + in_sequence, src);
+    t.all_tiles = key_tiles_of(a, t.position + t.count);
+    t.key_tiles = t.all_tiles;
+    t.slot = -1;
+    const int pass = unit % a.passes;
+    t.head = unit / a.passes;
+    t.head0 = t.head * a.group + pass * a.heads;
+    t.heads = min(a.heads, a.group - pass * a.heads);
+    if (lane == 0 && t.position + t.count > a.capacity) raise_status(a.status, kStatusBadIndex);
+    break;
   }
-  return Tile{0, 0, 0, 0};
+  return t;
+}
+
+// Inclusive sum over the CTA; `sums` holds one value per warp.
+Q3T_DEV int block_sum(int v, int* sums, int warp, int lane, int& all) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int other = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += other;
+  }
+  if (lane == 31) sums[warp] = v;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const int s = sums[w];
+    if (w < warp) v += s;
+    all += s;
+  }
+  __syncthreads();
+  return v;
+}
+
+// Where range `i` of `parts` begins among `total` units of work (an item: its key tiles and kFixed), moved
+// to an item's end where less than kLeast tiles would be cut off.
+Q3T_DEV int64_t range_begin(const int32_t* prefix, int pairs, int units, int64_t i, int64_t total, int64_t parts) {
+  const int64_t at = split_begin(i, total, parts);
+  if (at <= 0 || at >= total) return at;
+  const int e = row_of(prefix, pairs, at, units);
+  const int n = prefix[e + 1] - prefix[e];
+  const int64_t base = int64_t(prefix[e]) * units;
+  const int64_t item = base + (at - base) / n * n;
+  const int o = int(at - item);
+  // an item's fixed cost stands at its beginning
+  if (n < 2 * kLeast + kFixed ? 2 * o <= n : o < kLeast + kFixed) return item;
+  if (n < 2 * kLeast + kFixed || n - o < kLeast) return item + n;
+  return at;
 }
 
 template <int D>
@@ -225,271 +365,503 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kHalves = D / 64;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Bars* bars = reinterpret_cast<Bars*>(smem + M::kBar);
-  __shared__ Tile shared_tile;
+  Bars* bars = reinterpret_cast<Bars*>(smem + (M::kBar + 15) / 16 * 16);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = a.kv_heads * a.passes, unit = int(blockIdx.x % units), head = unit / a.passes;
-  const int head0 = head * a.group + unit % a.passes * a.heads;  // first query head
+  const int units = a.kv_heads * a.passes;
+  int given = 0;  // warp 3: segments handed out
   grid_dependency_wait();
-  if (warp == 0) {
-    const Tile found = find_tile(a, int(blockIdx.x / units), lane);
-    if (lane == 0) shared_tile = found;
-  } else if (warp == 1) {
+  if (warp == 3) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars->q_full[i], 1);
+        mbar_init(&bars->q_free[i], 1);
         mbar_init(&bars->s_full[i], 1);
         mbar_init(&bars->turn[i], 1);
         mbar_init(&bars->p_full[i][0], 128);
         mbar_init(&bars->p_full[i][1], 128);
         mbar_init(&bars->o_done[i], 1);
+        mbar_init(&bars->o_free[i], 128);
+        mbar_init(&bars->segment_full[i], 1);
+        mbar_init(&bars->segment_free[i], 10);  // warps that read it: loads, products, eight of softmax
       }
       for (int i = 0; i < kStages; ++i) {
         mbar_init(&bars->k_full[i], 1);
         mbar_init(&bars->v_full[i], 1);
       }
+      mbar_init(&bars->loaded, 1);
+      mbar_init(&bars->takeover, 1);
       mbar_init(&bars->done, 1);
       fence_mbar_init();
     }
-  }
-  __syncthreads();
-  const Tile tile = shared_tile;
-  if (tile.count == 0) return;
-  if (warp == 2) {
+    __syncwarp();
+    if (a.parts == 0) {  // the CTA's only item
+      const Segment seg = find_tile(a, int(blockIdx.x) / units, int(blockIdx.x) % units, lane);
+      if (lane == 0 && seg.count > 0) {
+        bars->segments[0] = seg;
+        mbar_arrive(&bars->segment_full[0]);
+      }
+      given = seg.count > 0;
+    }
+  } else if (warp == 2) {
     tmem_alloc(&bars->tmem, 512);
     tmem_relinquish();
+  } else if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tmq);
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
   }
-  // rows, last key + 1 and key tiles of each query tile; keys that the table cannot hold are cut off
-  int count[2], key_end[2], tiles[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    count[t] = max(0, min(a.positions, tile.count - t * a.positions));
-    const int64_t end = tile.position + t * a.positions + count[t];
-    if (count[t] > 0 && end > a.capacity && threadIdx.x == 0) raise_status(a.status, kStatusBadIndex);
-    key_end[t] = count[t] == 0 || end < 0 ? 0 : int(end < a.capacity ? end : a.capacity);
-    tiles[t] = (key_end[t] + kTileKeys - 1) / kTileKeys;
+  // ---- the plan: work before every query tile pair, for one unit
+  int32_t* prefix = reinterpret_cast<int32_t*>(smem + M::kPlan);
+  int pairs = 0;
+  if (a.parts > 0) {
+    int32_t* before = prefix + kPlanTiles + 1;  // pairs of the sequences after s: numbers begin at the last one
+    const int span = 2 * a.positions;
+    for (int s0 = 0; s0 < a.sequences; s0 += kThreads) {
+      const int s = a.sequences - 1 - s0 - int(threadIdx.x);
+      int first, n = s >= 0 ? rows_of(a, s, first) : 0, all;
+      n = (n + span - 1) / span;
+      const int sum = block_sum(n, bars->sums, warp, lane, all);
+      if (s >= 0) before[a.sequences - 1 - s] = pairs + sum - n;
+      pairs += all;
+    }
+    __syncthreads();
+    int work = 0;
+    for (int e0 = 0; e0 < pairs; e0 += kThreads) {
+      const int e = e0 + int(threadIdx.x);
+      int cost = 0, all;
+      if (e < pairs) {
+        const int i = row_of(before, a.sequences, e, 1), s = a.sequences - 1 - i;
+        int first;
+        const int n = rows_of(a, s, first), tile = (n + span - 1) / span - 1 - (e - before[i]);
+        cost = kFixed + key_tiles_of(a, a.start_positions[s] + min(n, (tile + 1) * span));
+      }
+      const int sum = block_sum(cost, bars->sums, warp, lane, all);
+      if (e < pairs) prefix[e] = work + sum - cost;
+      work += all;
+    }
+    if (threadIdx.x == 0) prefix[pairs] = work;
   }
-  const int key_tiles = max(tiles[0], tiles[1]), keys = max(key_end[0], key_end[1]);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
+
+  // the next segment of work, for one warp; false: none, or a wait gave up
+  int taken = 0;
+  auto take = [&](Segment& seg, bool& ok) {
+    ok = warp_wait(&bars->segment_full[taken & 1], taken >> 1, a.status, kStatusFlagTimeout);
+    if (!ok) return false;
+    seg = bars->segments[taken & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->segment_free[taken & 1]);
+    ++taken;
+    return seg.count > 0;
+  };
+  // rows and key tiles of each of its query tiles, and its keys, numbered from its first key tile on
+  auto shape = [&](const Segment& seg, int (&count)[2], int (&tiles)[2], int& keys) {
+    keys = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      count[t] = max(0, min(a.positions, seg.count - t * a.positions));
+      const int end = count[t] > 0 ? keys_of(a, seg.position + t * a.positions + count[t]) - seg.tile0 * kTileKeys : 0;
+      tiles[t] = max(0, min(seg.key_tiles, (end + kTileKeys - 1) / kTileKeys));
+      keys = max(keys, min(end, seg.key_tiles * kTileKeys));
+    }
+  };
+  int count[2], tiles[2], keys;
+  bool ok = true;
 
   if (warp >= 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ---------------- softmax: thread = query row = TMEM lane
     const int t = (warp >> 2) - 1, m = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t s_at = lanes + 128 * t, o_at = lanes + 256 + 128 * t;
-    const int p = m / a.heads, h = m % a.heads;
-    const bool real = p < count[t] && unit % a.passes * a.heads + h < a.group;
-    const int64_t position = tile.position + t * a.positions + p;
-    const int last = int(position < -1 ? -1 : position < a.capacity ? position : a.capacity - 1);  // last key seen
-    float top = -INFINITY, sum = 0.f;
-    bool ok = true;
-    for (int j = 0; j < tiles[t]; ++j) {
-      if (!warp_wait(&bars->s_full[t], j, a.status, kStatusMmaTimeout)) {
-        ok = false;
-        break;
+    const uint32_t s_at = lanes + 128 * t;  // this tile's scores and weights; its output 256 columns on
+    const int p = m / a.heads, h = m - p * a.heads;
+    int done = 0, outs = 0;  // key tiles and outputs so far
+    for (;; ++taken) {
+      ok = warp_wait(&bars->segment_full[taken & 1], taken >> 1, a.status, kStatusFlagTimeout);
+      // read where it stands, and again after the key tiles: their loop needs every register
+      const Segment& seg = bars->segments[taken & 1];
+      if (!ok || seg.count == 0) break;
+      int key_tiles, seen0;  // of this query tile; keys that the row sees from the segment's first on
+      {
+        shape(seg, count, tiles, keys);
+        key_tiles = tiles[t];
+        const int64_t position = seg.position + t * a.positions + p;
+        seen0 = int(position < -1 ? -1 : position < a.capacity ? position : a.capacity - 1) + 1 - seg.tile0 * kTileKeys;
       }
-      tc_fence_after();
-      float s[128];
+      float top = -INFINITY, sum = 0.f;
+      for (int j = 0; j < key_tiles; ++j, ++done) {
+        if (!warp_wait(&bars->s_full[t], done, a.status, kStatusMmaTimeout)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float s[128];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, s + 32 * c);
-      tmem_ld_wait();
-      const int seen = last + 1 - j * kTileKeys;  // keys of this tile that the row sees
-      if (__any_sync(0xffffffffu, seen < kTileKeys)) {
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + 32 * c, s + 32 * c);
 #pragma unroll
-        for (int i = 0; i < 128; ++i) s[i] = i < seen ? s[i] : -INFINITY;
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        for (int c = 0; c < 4; ++c) c == 0 ? tmem_ld_wait<true>(s) : tmem_ld_wait<false>(s + 32 * c);
+        const int seen = seen0 - j * kTileKeys;  // keys of this tile that the row sees
+        if (__any_sync(0xffffffffu, seen < kTileKeys)) {
 #pragma unroll
-      for (int i = 0; i < 128; i += 2) mx[i / 2 & 3] = max3(mx[i / 2 & 3], s[i], s[i + 1]);
-      const float now = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-      if (__any_sync(0xffffffffu, now > top + 8.f || (top == -INFINITY && now > top))) {
-        const float to = fmaxf(top, now);
-        const float f = to == top ? 1.f : exp2_fast(top - to);
-        top = to;
-        sum *= f;
-        if (j > 0) {  // the products up to tile j - 1 are done: s_full says so
+          for (int i = 0; i < 128; ++i) s[i] = i < seen ? s[i] : -INFINITY;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            tmem_ld32(o_at + 32 * c, o);
-            tmem_ld_wait();
+        for (int i = 0; i < 128; i += 2) mx[i / 2 & 3] = max3(mx[i / 2 & 3], s[i], s[i + 1]);
+        const float now = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+        if (__any_sync(0xffffffffu, now > top + 8.f || (top == -INFINITY && now > top))) {
+          const float to = fmaxf(top, now);
+          const float f = to == top ? 1.f : exp2_fast(top - to);
+          top = to;
+          sum *= f;
+          if (j > 0) {  // the products up to tile j - 1 are done: s_full says so
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              float o[16];
+              tmem_ld16(s_at + 256 + c, o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= f;
-            tmem_st32(o_at + 32 * c, reinterpret_cast<const uint32_t*>(o));
+              for (int i = 0; i < 16; ++i) o[i] *= f;
+              tmem_st16(s_at + 256 + c, reinterpret_cast<const uint32_t*>(o));
+            }
           }
         }
-      }
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
-      float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
+        const float ref = top == -INFINITY ? 0.f : top;
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
+        float2 part[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
+        for (int quarter = 0; quarter < 4; ++quarter) {
+          uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float2 x = fma2(make_float2(s[64 * c + 2 * i], s[64 * c + 2 * i + 1]), scale2, ref2);
-          x.x = exp2_fast(x.x);
-          x.y = exp2_fast(x.y);
-          part[i & 1] = add2(part[i & 1], x);
-          w[i] = pack2(x.x, x.y);
+          for (int i = 0; i < 16; ++i) {
+            float2 x = fma2(make_float2(s[32 * quarter + 2 * i], s[32 * quarter + 2 * i + 1]), scale2, ref2);
+            if ((i & 7) == 3) {  // one in eight: 2 % (D = 128) to 8 % (64); one in four is no faster, one in two slower
+              x = exp2_poly(x);
+            } else {
+              x.x = exp2_fast(x.x);
+              x.y = exp2_fast(x.y);
+            }
+            part[i & 1] = add2(part[i & 1], x);
+            w[i] = pack2(x.x, x.y);
+          }
+          tmem_st16(s_at + 16 * quarter, w);
+          if (quarter & 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&bars->p_full[t][quarter >> 1]);
+          }
         }
-        tmem_st32(s_at + 32 * c, w);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&bars->p_full[t][c]);
+        sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
       }
-      sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-    }
-    // ---- O / l
-    if (tiles[t] > 0) ok = ok && warp_wait(&bars->o_done[t], 0, a.status, kStatusMmaTimeout);
-    tc_fence_after();
-    __nv_bfloat16* to = a.out + (int64_t(tile.row + t * a.positions + p) * a.q_heads + head0 + h) * D;
-    const float inv = last < 0 ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-      float o[32];
-      if (tiles[t] > 0 && ok) {  // uniform over the warp
-        tmem_ld32(o_at + 32 * c, o);
-        tmem_ld_wait();
+      if (ok && key_tiles > 0) {
+        ok = warp_wait(&bars->o_done[t], outs, a.status, kStatusMmaTimeout);
+        ++outs;
       }
-      if (real && ok) {
+      if (!ok) break;
+      tc_fence_after();
+      const bool none = seg.position + t * a.positions + p < 0;  // the row sees nothing
+      if (seg.slot < 0) {
+        // ---- O / l: each thread its row, a whole sector (16 dims) a store. A row without keys is 0; a maximum of +inf
+        // leaves no value.
+        const float inv = none ? 0.f : top == INFINITY ? NAN : 1.f / sum;
+        const bool real = p < min(a.positions, seg.count - t * a.positions) && h < seg.heads;
+        __nv_bfloat16* to = a.out + ((int64_t(seg.row) + t * a.positions + p) * a.q_heads + seg.head0 + h) * D;
+#pragma unroll 1  // the code runs once an item: short is faster than unrolled, which waits for its instructions
+        for (int c = 0; c < D / 32; ++c, to += 32) {
+          float o[32];
+          if (key_tiles > 0) {  // uniform over the warp
+            tmem_ld32(s_at + 256 + 32 * c, o);
+            tmem_ld_wait(o);
+          }
+          uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = last < 0 ? 0.f : o[8 * i + e] * inv;
-          *reinterpret_cast<uint4*>(to + 32 * c + 8 * i) = pack8(v);
+          for (int i = 0; i < 16; ++i) w[i] = none ? 0u : pack2(o[2 * i] * inv, o[2 * i + 1] * inv);
+          if (real) {
+            store32(to, w, a.out_32);
+            store32(to + 16, w + 8, a.out_32);
+          }
         }
+      } else {
+        float* part = a.partial + (int64_t(blockIdx.x) * 2 + seg.slot) * kPartFloats<D>;
+        const int row = t * 128 + m;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (key_tiles > 0) {
+            tmem_ld32(s_at + 256 + 32 * c, o);
+            tmem_ld_wait(o);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<float4*>(part + ((8 * c + i) * 256 + row) * 4) =
+                key_tiles > 0 ? make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        *reinterpret_cast<float2*>(part + 256 * D + 2 * row) = make_float2(top, sum);
       }
+      tc_fence_before();
+      if (key_tiles > 0) mbar_arrive(&bars->o_free[t]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->segment_free[taken & 1]);
     }
     tc_fence_before();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
-  if (warp == 0) {
-    // ---------------- loads
-    bool ok = true;
-    if (lane == 0) {
-      for (int t = 0; t < 2; ++t) {
-        if (tiles[t] == 0) continue;
-        mbar_expect_tx(&bars->q_full[t], uint32_t(a.heads * a.positions * 128 * kHalves));
-        for (int h = 0; h < kHalves; ++h)
-          tma_load_3d(smem + t * M::kTile + h * M::kBlock, &tmq, &bars->q_full[t], h * 64, head0,
-                      tile.row + t * a.positions, policy_evict_first());
-      }
-    }
-    // lane: (piece of the tile, 64-dim block)
-    const int pieces = kTileKeys / a.piece, piece = lane / kHalves, half = lane % kHalves;
-    auto page_of = [&](int j) {  // the page of this lane's piece of tile j, and its row there
-      int2 at = make_int2(int(a.pages.pages), 0);  // past the pool: a load of zeros
-      const int key = j * kTileKeys + piece * a.piece;
-      if (piece < pieces && key < keys) {
-        const int64_t page = a.pages.lookup(tile.sequence, key);
-        if (page >= 0) at = make_int2(int(page), key % a.pages.page_size);
-        else raise_status(a.status, kStatusBadIndex);
-      }
-      return at;
-    };
-    int2 next = page_of(0);
-    int loaded = 0;
-    for (int j = 0; j < key_tiles && ok; ++j) {
-      const int s = j % kStages;
-      const int2 at = next;
-      const int wanted = min(pieces, (keys - j * kTileKeys + a.piece - 1) / a.piece);  // pieces that hold a key
-      const uint32_t bytes = uint32_t(wanted * a.piece * 128 * kHalves);
-#pragma unroll
-      for (int v = 0; v < 2 && ok; ++v) {
-        // turn i of the products has read key tile i and value tile i - 1
-        const int turn = j - kStages + v;
-        if (j >= kStages) ok = warp_wait(&bars->turn[turn & 1], turn >> 1, a.status, kStatusMmaTimeout);
-        if (!ok) break;
-        uint64_t* full = v ? &bars->v_full[s] : &bars->k_full[s];
-        if (lane == 0) mbar_expect_tx(full, bytes);
-        __syncwarp();
-        if (piece < wanted)
-          tma_load_4d(smem + (v ? M::kV : M::kK) + s * M::kTile + half * M::kBlock + piece * a.piece * 128, v ? &tmv : &tmk,
-                      full, half * 64, at.y, head, at.x);
-        ++loaded;
-      }
-      if (j + 1 < key_tiles) next = page_of(j + 1);
-    }
-    if (!ok)  // loads still in flight land before the CTA leaves
-      for (int i = max(0, loaded - 2 * kStages); i < loaded; ++i)
-        mbar_wait(i & 1 ? &bars->v_full[(i / 2) % kStages] : &bars->k_full[(i / 2) % kStages], (i / 2 / kStages) & 1, a.status,
-                  kStatusTmaTimeout);
-  } else if (warp == 1) {
-    // ---------------- products (TMEM column 0 is the allocation's first: it is all of TMEM)
-    constexpr uint32_t idesc_s = umma_idesc_bf16(128, kTileKeys);
-    constexpr uint32_t idesc_o = umma_idesc_bf16(128, D) | (1u << 16);  // V MN-major
-    const uint32_t base = smem_u32(smem);
-    const bool leader = elect_one();
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, int phase, unsigned bit) { ok = ok && warp_wait(bar, phase, a.status, bit); };
-    auto scores = [&](int t, int s) {
-      const uint32_t q = desc_k(base + t * M::kTile), k = desc_k(base + M::kK + s * M::kTile);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint32_t step = (i >> 2) * (M::kBlock >> 4) + 2 * (i & 3);
-        mma_ss(128 * t, q + step, k + step, idesc_s, i > 0, leader);
-      }
-      commit_if(&bars->s_full[t], leader);
-    };
-    if (key_tiles > 0) {
-      wait(&bars->k_full[0], 0, kStatusTmaTimeout);
-      for (int t = 0; t < 2; ++t) {
-        if (tiles[t] == 0) continue;
-        wait(&bars->q_full[t], 0, kStatusTmaTimeout);
-        tc_fence_after();
-        if (ok) scores(t, 0);
-      }
-      if (ok) commit_if(&bars->turn[0], leader);
-    }
-    for (int j = 0; j < key_tiles && ok; ++j) {
-      const int s = j % kStages, phase = j / kStages, sn = (j + 1) % kStages;
-      wait(&bars->v_full[s], phase, kStatusTmaTimeout);
-      const int valid = keys - j * kTileKeys;
-      if (ok && valid < kTileKeys) {
-        // value rows past the last key hold anything, or were not loaded: their weights are 0, and 0 * NaN is NaN
-        for (int e = lane; e < (kTileKeys - valid) * 8 * kHalves; e += 32) {
-          const int h = e % kHalves, c = e / kHalves;
-          *reinterpret_cast<uint4*>(smem + M::kV + s * M::kTile + h * M::kBlock + valid * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+    Segment seg;
+    if (warp == 0) {
+      // ---------------- loads. Lane: (piece of a key tile, 64-dim block)
+      const int pieces = kTileKeys / a.piece, piece = lane / kHalves, half = lane % kHalves;
+      int n = 0, loaded = 0, queries[2] = {0, 0};  // key tiles so far; loads begun; query tiles so far
+      while (ok && take(seg, ok)) {
+        shape(seg, count, tiles, keys);
+        const int key0 = seg.tile0 * kTileKeys;
+        auto page_of = [&](int j) {  // the page of this lane's piece of tile j, and its row there
+          int2 at = make_int2(int(a.pages.pages), 0);  // past the pool: a load of zeros
+          const int key = j * kTileKeys + piece * a.piece;
+          if (piece < pieces && key < keys) {
+            const int64_t page = a.pages.lookup(seg.sequence, key0 + key);
+            if (page >= 0) at = make_int2(int(page), (key0 + key) % a.pages.page_size);
+            else raise_status(a.status, kStatusBadIndex);
+          }
+          return at;
+        };
+        int2 next = page_of(0);
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (tiles[t] == 0) continue;
+          if (queries[t] > 0) ok = warp_wait(&bars->q_free[t], queries[t] - 1, a.status, kStatusMmaTimeout);
+          if (!ok) break;
+          ++queries[t];
+          if (lane == 0) {
+            mbar_expect_tx(&bars->q_full[t], uint32_t(a.heads * a.positions * 128 * kHalves));
+            for (int h = 0; h < kHalves; ++h)
+              tma_load_3d(smem + t * M::kTile + h * M::kBlock, &tmq, &bars->q_full[t], h * 64,
+                          seg.head0, seg.row + t * a.positions, policy_evict_first());
+          }
         }
-        fence_async_shared();
-        __syncwarp();
+        for (int j = 0; j < seg.key_tiles && ok; ++j, ++n) {
+          const int s = n % kStages;
+          const int2 at = next;
+          const int wanted = min(pieces, (keys - j * kTileKeys + a.piece - 1) / a.piece);  // pieces that hold a key
+          const uint32_t bytes = uint32_t(wanted * a.piece * 128 * kHalves);
+#pragma unroll
+          for (int v = 0; v < 2 && ok; ++v) {
+            // turn i of the products has read key tile i and value tile i - 1
+            const int turn = n - kStages + v;
+            if (n >= kStages) ok = warp_wait(&bars->turn[turn & 1], turn >> 1, a.status, kStatusMmaTimeout);
+            if (!ok) break;
+            uint64_t* full = v ? &bars->v_full[s] : &bars->k_full[s];
+            if (lane == 0) mbar_expect_tx(full, bytes);
+            __syncwarp();
+            if (piece < wanted)
+              tma_load_4d(smem + (v ? M::kV : M::kK) + s * M::kTile + half * M::kBlock + piece * a.piece * 128, v ? &tmv : &tmk,
+                          full, half * 64, at.y, seg.head, at.x);
+            ++loaded;
+          }
+          if (j + 1 < seg.key_tiles) next = page_of(j + 1);
+        }
+        if (lane == 0) mbar_arrive(&bars->loaded);
       }
-      if (j + 1 < key_tiles) wait(&bars->k_full[sn], (j + 1) / kStages, kStatusTmaTimeout);
-      const uint32_t v = desc_mn(base + M::kV + s * M::kTile, M::kBlock);
+      if (!ok) {  // loads still in flight land before the CTA leaves
+        for (int t = 0; t < 2; ++t)
+          if (queries[t] > 0) mbar_wait(&bars->q_full[t], (queries[t] - 1) & 1, a.status, kStatusTmaTimeout);
+        for (int i = max(0, loaded - 2 * kStages); i < loaded; ++i)
+          mbar_wait(i & 1 ? &bars->v_full[(i / 2) % kStages] : &bars->k_full[(i / 2) % kStages], (i / 2 / kStages) & 1, a.status,
+                    kStatusTmaTimeout);
+      }
+    } else if (warp == 1) {
+      // ---------------- products (TMEM column 0 is the allocation's first: it is all of TMEM)
+      constexpr uint32_t idesc_s = umma_idesc_bf16(128, kTileKeys);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(128, D) | (1u << 16);  // V MN-major
+      const uint32_t base = smem_u32(smem);
+      const bool leader = elect_one();
+      int n = 0, weights[2] = {0, 0}, queries[2] = {0, 0};  // key tiles, weight tiles and query tiles so far
+      auto wait = [&](uint64_t* bar, int phase, unsigned bit) { ok = ok && warp_wait(bar, phase, a.status, bit); };
+      auto scores = [&](int t, int s) {
+        const uint32_t q = desc_k(base + t * M::kTile), k = desc_k(base + M::kK + s * M::kTile);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (j >= tiles[t]) continue;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // the first 64 keys' weights come before the others are computed
-          wait(&bars->p_full[t][half], j, kStatusMmaTimeout);
+        for (int i = 0; i < D / 16; ++i) {
+          const uint32_t step = (i >> 2) * (M::kBlock >> 4) + 2 * (i & 3);
+          mma_ss(128 * t, q + step, k + step, idesc_s, i > 0, leader);
+        }
+        commit_if(&bars->s_full[t], leader);
+      };
+      while (ok && take(seg, ok)) {
+        shape(seg, count, tiles, keys);
+        const int key_tiles = __shfl_sync(0xffffffffu, seg.key_tiles, 0);  // so that the compiler knows them uniform
+        tiles[0] = __shfl_sync(0xffffffffu, tiles[0], 0);
+        tiles[1] = __shfl_sync(0xffffffffu, tiles[1], 0);
+        keys = __shfl_sync(0xffffffffu, keys, 0);
+        if (key_tiles == 0) continue;
+        wait(&bars->k_full[n % kStages], n / kStages, kStatusTmaTimeout);
+        for (int t = 0; t < 2; ++t) {
+          if (tiles[t] == 0) continue;
+          wait(&bars->q_full[t], queries[t], kStatusTmaTimeout);
           tc_fence_after();
-          if (!ok) continue;
-#pragma unroll
-          for (int i = 4 * half; i < 4 * half + 4; ++i)
-            mma_ts(256 + 128 * t, 128 * t + 8 * i, v + 128 * i, idesc_o, j > 0 || i > 0, leader);
+          if (!ok) break;
+          scores(t, n % kStages);
+          if (tiles[t] == 1) commit_if(&bars->q_free[t], leader);
         }
-        if (!ok) continue;
-        if (j + 1 < tiles[t]) scores(t, sn);
-        else commit_if(&bars->o_done[t], leader);
+        if (ok) commit_if(&bars->turn[n & 1], leader);
+        for (int j = 0; j < key_tiles && ok; ++j, ++n) {
+          const int s = n % kStages, sn = (n + 1) % kStages;
+          wait(&bars->v_full[s], n / kStages, kStatusTmaTimeout);
+          const int valid = keys - j * kTileKeys;
+          if (ok && valid < kTileKeys) {
+            // value rows past the last key hold anything, or were not loaded: their weights are 0, and 0 * NaN is NaN
+            for (int e = lane; e < (kTileKeys - valid) * 8 * kHalves; e += 32) {
+              const int h = e % kHalves, c = e / kHalves;
+              *reinterpret_cast<uint4*>(smem + M::kV + s * M::kTile + h * M::kBlock + valid * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_shared();
+            __syncwarp();
+          }
+          const uint32_t v = desc_mn(base + M::kV + s * M::kTile, M::kBlock);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= tiles[t]) continue;
+            // the last output of this query tile has been read
+            if (j == 0 && queries[t] > 0) wait(&bars->o_free[t], queries[t] - 1, kStatusMmaTimeout);
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {  // the first 64 keys' weights come before the others are computed
+              wait(&bars->p_full[t][part], weights[t], kStatusMmaTimeout);
+              tc_fence_after();
+              if (!ok) continue;
+#pragma unroll
+              for (int i = 4 * part; i < 4 * part + 4; ++i)
+                mma_ts(256 + 128 * t, 128 * t + 8 * i, v + 128 * i, idesc_o, j > 0 || i > 0, leader);
+            }
+            if (!ok) continue;
+            ++weights[t];
+            if (j + 1 < tiles[t]) {
+              wait(&bars->k_full[sn], (n + 1) / kStages, kStatusTmaTimeout);  // behind the products just issued
+              if (!ok) continue;
+              scores(t, sn);
+              if (j + 2 == tiles[t]) commit_if(&bars->q_free[t], leader);
+            } else {
+              commit_if(&bars->o_done[t], leader);
+            }
+          }
+          if (ok && j + 1 < key_tiles) commit_if(&bars->turn[(n + 1) & 1], leader);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) queries[t] += tiles[t] > 0;
       }
-      if (ok) commit_if(&bars->turn[(j + 1) & 1], leader);
+      if (lane == 0) {  // every product is done before TMEM is released
+        umma_commit(&bars->done);
+        mbar_wait(&bars->done, 0, a.status, kStatusMmaTimeout);
+      }
+    } else if (warp == 3) {
+      // ---------------- work
+      auto give = [&](const Segment& g) {
+        if (given >= 2) ok = warp_wait(&bars->segment_free[given & 1], (given >> 1) - 1, a.status, kStatusFlagTimeout);
+        if (!ok) return;
+        if (lane == 0) {
+          bars->segments[given & 1] = g;
+          mbar_arrive(&bars->segment_full[given & 1]);  // releases what the lane wrote
+        }
+        ++given;
+      };
+      if (a.parts == 0) {
+        // The first item was handed out above. More: take over CTAs of this grid that have not been launched yet, so the
+        // items still go to the SMs one by one, as those get free: asked for when an item's last loads are out.
+        int items = given;
+        for (int i = 0; ok; ++i) {
+          if (items > 0) ok = warp_wait(&bars->loaded, items - 1, a.status, kStatusFlagTimeout);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_expect_tx(&bars->takeover, 16);
+            try_take_over(&bars->response, &bars->takeover);
+          }
+          ok = warp_wait(&bars->takeover, i, a.status, kStatusFlagTimeout);
+          int block = 0;
+          if (!ok || !taken_over(&bars->response, block)) break;
+          seg = find_tile(a, block / units, block % units, lane);
+          if (seg.count > 0) {
+            give(seg);
+            ++items;
+          }
+        }
+      } else {
+        Segment left[2] = {};  // what this range leaves to the join
+        const int64_t total = int64_t(prefix[pairs]) * units;
+        const int64_t parts = split_parts(total / kLeast > 1 ? total / kLeast : 1, a.parts);
+        const int64_t f1 = int64_t(blockIdx.x) < parts ? range_begin(prefix, pairs, units, blockIdx.x + 1, total, parts) : 0;
+        int64_t f = int64_t(blockIdx.x) < parts ? range_begin(prefix, pairs, units, blockIdx.x, total, parts) : 0;
+        while (f < f1 && ok) {
+          const int e = row_of(prefix, pairs, f, units), n = prefix[e + 1] - prefix[e];
+          const int64_t base = int64_t(prefix[e]) * units;
+          const int unit = int((f - base) / n);
+          const int64_t item = base + int64_t(unit) * n, end = item + n < f1 ? item + n : f1;
+          seg = find_tile(a, e, unit, lane);
+          seg.tile0 = f > item ? int(f - item) - kFixed : 0;
+          seg.key_tiles = int(end - item) - kFixed - seg.tile0;
+          seg.slot = f > item ? 0 : end < item + n ? 1 : -1;
+          if (seg.slot >= 0) left[seg.slot] = seg;
+          if (seg.count > 0) give(seg);
+          f = end;
+        }
+        if (lane == 0) {
+          a.shared_segments[blockIdx.x * 2] = left[0];
+          a.shared_segments[blockIdx.x * 2 + 1] = left[1];
+        }
+      }
+      if (ok) give(Segment{});
     }
-    if (lane == 0) {  // every product is done before TMEM is released
-      umma_commit(&bars->done);
-      mbar_wait(&bars->done, 0, a.status, kStatusMmaTimeout);
-    }
-  }
   }
   __syncthreads();
   if (warp == 2) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of an item that several ranges share: CTA (i, quarter) the 64 rows of the item that range i began and
+// did not end.
+template <int D>
+__global__ void __launch_bounds__(256) paged_prefill_join(const PrefillArgs a) {
+  grid_dependency_wait();
+  const Segment first = a.shared_segments[blockIdx.x * 2 + 1];
+  if (first.count == 0) return;
+  const int row = blockIdx.y * 64 + (threadIdx.x & 63), chunk0 = (threadIdx.x >> 6) * (D / 16);  // of D / 4
+  const int t = row >> 7, p = (row & 127) / a.heads, h = (row & 127) % a.heads;
+  const int count = max(0, min(a.positions, first.count - t * a.positions));
+  if (p >= count || h >= first.heads) return;
+  // parts: slot 1 of this range, then slot 0 of the next ones up to the item's end
+  auto part_of = [&](int i) { return a.partial + (int64_t(blockIdx.x + i) * 2 + (i == 0)) * kPartFloats<D>; };
+  float top = -INFINITY;
+  int parts = 0;
+  for (int end = first.key_tiles;; ++parts) {
+    top = fmaxf(top, part_of(parts)[256 * D + 2 * row]);
+    if (end >= first.all_tiles || int(blockIdx.x) + parts + 1 >= a.parts) break;
+    const Segment& next = a.shared_segments[(blockIdx.x + parts + 1) * 2];
+    end = next.tile0 + next.key_tiles;
+  }
+  ++parts;
+  float l = 0.f, v[D / 4] = {};
+  for (int i = 0; i < parts; ++i) {
+    const float* part = part_of(i);
+    const float2 ml = *reinterpret_cast<const float2*>(part + 256 * D + 2 * row);
+    const float f = ml.x == top ? 1.f : exp2_fast(ml.x - top);
+    l += ml.y * f;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const float4 o = *reinterpret_cast<const float4*>(part + ((chunk0 + c) * 256 + row) * 4);
+      v[4 * c] += o.x * f;
+      v[4 * c + 1] += o.y * f;
+      v[4 * c + 2] += o.z * f;
+      v[4 * c + 3] += o.w * f;
+    }
+  }
+  const bool none = first.position + t * a.positions + p < 0;
+  const float inv = top == INFINITY ? NAN : 1.f / l;
+  __nv_bfloat16* out = a.out + (int64_t(first.row + t * a.positions + p) * a.q_heads + first.head0 + h) * D + chunk0 * 4;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = none ? 0.f : v[8 * c + e] * inv;
+    *reinterpret_cast<uint4*>(out + 8 * c) = pack8(w);
   }
 }
 
@@ -507,8 +879,36 @@ int launch_prefill(const q3t_paged_prefill& p, const PrefillArgs& a, int64_t blo
       return rc;
   static PerDevice once;
   if (const int rc = smem_limit(once, paged_prefill_kernel<D>, Smem<D>::kBytes, name)) return rc;
-  return launch(paged_prefill_kernel<D>, dim3(unsigned(blocks)), dim3(kThreads), size_t(Smem<D>::kBytes), stream, true, name,
-                tmq, tmk, tmv, a);
+  if (const int rc = launch(paged_prefill_kernel<D>, dim3(unsigned(blocks)), dim3(kThreads), size_t(Smem<D>::kBytes), stream,
+                            true, name, tmq, tmk, tmv, a))
+    return rc;
+  if (a.parts == 0) return Q3T_OK;
+  return launch(paged_prefill_join<D>, dim3(unsigned(a.parts), 4), dim3(256), 0, stream, true, name, a);
+}
+
+// How a call runs, from sizes that the host knows.
+struct PrefillPlan {
+  int heads, passes, positions;
+  int64_t items;  // at most: every sequence may end inside a pair of tiles
+  int parts;      // ranges; 0: one item per CTA
+  size_t bytes;
+};
+PrefillPlan prefill_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t capacity) {
+  PrefillPlan p;
+  const int64_t group = q_heads / kv_heads;
+  p.heads = int(group < 64 ? group : 64);
+  p.passes = int((group + p.heads - 1) / p.heads);
+  p.positions = kTileRows / p.heads;
+  const int64_t pairs = rows / (2 * p.positions) + sequences;
+  p.items = pairs * kv_heads * p.passes;
+  // Ranges pay where items are few and may be long: 4 chunks of 100..700 rows behind 2000..8000 keys 148 us in turn, 117 in
+  // ranges; 512 rows behind 16000 keys 221 and 77; 1 row behind 2000 keys 30 and 24. With many items they only add the
+  // plan and the join (one prompt of 4096 rows and 32 heads: 128 and 137; one of 2048 and 16 heads: 36 and 44).
+  const int64_t tiles = (capacity + kTileKeys - 1) / kTileKeys, sms = sm_count();
+  const bool few = (tiles >= 32 && p.items <= 3 * sms) || (tiles >= 16 && p.items <= sms / 4);
+  p.parts = few && pairs <= kPlanTiles && sequences <= kPlanSequences && pairs * (tiles + kFixed) < (int64_t(1) << 31) ? int(sms) : 0;
+  p.bytes = p.parts == 0 ? 0 : size_t(p.parts) * 2 * (sizeof(Segment) + size_t(256) * (head_dim + 2) * 4);
+  return p;
 }
 
 }  // namespace
@@ -520,8 +920,17 @@ bool prefill_tiles_supported(const q3t_paged_prefill& p) {
   return p.scale > 0. && p.scale < 1e30 && c.table_columns * c.page_size < (int64_t(1) << 30) && p.rows < (int64_t(1) << 28);
 }
 
+size_t prefill_tiles_workspace(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                               int64_t capacity) {
+  return prefill_plan(rows, sequences, q_heads, kv_heads, head_dim, capacity).bytes;
+}
+
 int launch_prefill_tiles(const q3t_paged_prefill& p, unsigned* status, void* stream, const char* name) {
   const q3t_paged_cache& c = p.cache;
+  const PrefillPlan plan = prefill_plan(p.rows, p.sequences, p.q_heads, c.kv_heads, c.head_dim, c.table_columns * c.page_size);
+  if (plan.bytes > 0 && (p.workspace == nullptr || p.workspace_bytes < int64_t(plan.bytes) || !aligned16(p.workspace)))
+    return fail(Q3T_ESPACE, "%s: workspace of %zu bytes (16-byte aligned) needed", name, plan.bytes);
+  if (plan.items > 2147483647) return fail(Q3T_EINVAL, "%s: too many rows", name);
   PrefillArgs a;
   a.pages = PageTable{c.page_table, c.table_stride, c.table_rows, c.table_columns, c.pages, int(c.page_size)};
   a.row_offsets = p.row_offsets;
@@ -532,17 +941,20 @@ int launch_prefill_tiles(const q3t_paged_prefill& p, unsigned* status, void* str
   a.q_heads = int(p.q_heads);
   a.kv_heads = int(c.kv_heads);
   a.group = int(p.q_heads / c.kv_heads);
-  a.heads = a.group < 64 ? a.group : 64;
-  a.passes = (a.group + a.heads - 1) / a.heads;
-  a.positions = kTileRows / a.heads;
+  a.heads = plan.heads;
+  a.passes = plan.passes;
+  a.positions = plan.positions;
   a.piece = 16;
   while (a.piece < kTileKeys && c.page_size % (2 * a.piece) == 0) a.piece *= 2;
   a.capacity = int(c.table_columns * c.page_size);
   a.scale_log2 = float(p.scale) * kLog2e;
   a.status = status;
-  // every sequence may end inside a tile
-  const int64_t tiles = p.rows / (2 * a.positions) + p.sequences, blocks = tiles * a.kv_heads * a.passes;
-  if (blocks > 2147483647) return fail(Q3T_EINVAL, "%s: too many rows", name);
+  a.out_32 = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
+  a.items = int(plan.items);
+  a.parts = plan.parts;
+  a.shared_segments = static_cast<Segment*>(p.workspace);
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + size_t(plan.parts) * 2 * sizeof(Segment));
+  const int64_t blocks = plan.parts > 0 ? plan.parts : plan.items;
   return c.head_dim == 128 ? launch_prefill<128>(p, a, blocks, stream, name) : launch_prefill<64>(p, a, blocks, stream, name);
 }
 

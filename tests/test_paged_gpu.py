@@ -313,7 +313,22 @@ def test_prompt_long(ops, cuda):
     check_prompt(ops, cuda, 2, 2, 64, 16, [1500], [0], strided=True)
 
 
+@pytest.mark.parametrize("counts,starts", [([1], [5000]), ([90, 3], [3000, 0]), ([64, 1, 500], [4000, 9000, 0]),
+                                           ([40] * 9, [700] * 9), ([33], [-20]), ([20], [-40]),
+                                           ([2000, 1, 300, 0, 1111], [0, 3, 2000, 5, 77])])
+@pytest.mark.parametrize("q,kv,d,page", [(16, 8, 128, 64), (8, 8, 64, 16), (16, 1, 128, 48), (6, 1, 64, 256)])
+def test_prompt_ranges(ops, cuda, counts, starts, q, kv, d, page):
+    """Tables that could hold long contexts: the key tiles of all items in even ranges, some items in parts."""
+    check_prompt(ops, cuda, q, kv, d, page, counts, starts, columns=(1 << 17) // page + 1, lead=1, tail=1)
+
+
+def test_prompt_wide_groups(ops, cuda):
+    check_prompt(ops, cuda, 70, 1, 64, 16, [5, 40], [0, 3])
+    check_prompt(ops, cuda, 70, 1, 64, 16, [5, 40], [0, 3], columns=1000)
+
+
 def test_prompt_many_sequences(ops, cuda):
+    check_prompt(ops, cuda, 4, 2, 128, 16, [(7 * i) % 4 for i in range(1500)], [(5 * i) % 23 for i in range(1500)])
     check_prompt(ops, cuda, 4, 2, 128, 16, [(13 * i) % 41 for i in range(120)], [(5 * i) % 23 for i in range(120)])
 
 
