@@ -333,12 +333,13 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
     int64_t at = 0;
     if (i + lane < count) {
       const int64_t p0 = (first + i + lane) * kStepKeys;
-      int64_t page = a.pages.lookup(sequence, p0);
+      int row_there;
+      int64_t page = a.pages.lookup(sequence, p0, row_there);
       if (page < 0) {
         raise_status(a.status, kStatusBadIndex);
         page = 0;
       }
-      at = page * a.page_stride + (int64_t(head) * a.pages.page_size + p0 % a.pages.page_size) * D;
+      at = page * a.page_stride + (int64_t(head) * a.pages.page_size + row_there) * D;
     }
     return at;
   };

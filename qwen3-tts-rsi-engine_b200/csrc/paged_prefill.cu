@@ -620,8 +620,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           int2 at = make_int2(int(a.pages.pages), 0);  // past the pool: a load of zeros
           const int key = j * kTileKeys + piece * a.piece;
           if (piece < pieces && key < keys) {
-            const int64_t page = a.pages.lookup(seg.sequence, key0 + key);
-            if (page >= 0) at = make_int2(int(page), (key0 + key) % a.pages.page_size);
+            int row;
+            const int64_t page = a.pages.lookup(seg.sequence, key0 + key, row);
+            if (page >= 0) at = make_int2(int(page), row);
             else raise_status(a.status, kStatusBadIndex);
           }
           return at;

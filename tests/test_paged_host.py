@@ -26,13 +26,18 @@ int main() {
   // page table look-ups: in range, and every kind of miss; entries that are not needed are never read
   const int32_t table[3 * 5] = {7, 0, 3, 9, 9, 1, -1, 8, 2147483647, 9, -2147483647 - 1, 4, 6, 5, 9};
   PageTable t = {table, 5, 3, 4, 8, 48};  // 3 sequences, 4 of 5 columns in use, 8 pages of 48 positions
-  CHECK(t.lookup(0, 0) == 7 && t.lookup(0, 47) == 7 && t.lookup(0, 48) == 0 && t.lookup(0, 143) == 3);
-  CHECK(t.lookup(0, 144) == -1);   // page 9 of 8
-  CHECK(t.lookup(0, 192) == -1);   // past the columns
-  CHECK(t.lookup(1, 48) == -1 && t.lookup(1, 96) == -1 && t.lookup(1, 144) == -1 && t.lookup(2, 0) == -1);
-  CHECK(t.lookup(2, 50) == 4 && t.lookup(2, -1) == -1);
-  CHECK(t.lookup(-1, 0) == -1 && t.lookup(3, 0) == -1 && t.lookup(int64_t(1) << 62, 0) == -1);
-  CHECK(t.lookup(0, int64_t(1) << 62) == -1 && t.lookup(0, -(int64_t(1) << 62)) == -1);
+  int row;
+  auto look = [&](int64_t s, int64_t p) { return t.lookup(s, p, row); };
+  CHECK(look(0, 143) == 3 && row == 47 && look(2, 50) == 4 && row == 2 && look(0, 48) == 0 && row == 0);
+  for (int64_t p : {int64_t(0), int64_t(47), int64_t(4294967295), int64_t(4294967296), int64_t(1) << 50})
+    CHECK(t.column_of(p) == p / 48);
+  CHECK(look(0, 0) == 7 && look(0, 47) == 7 && look(0, 48) == 0 && look(0, 143) == 3);
+  CHECK(look(0, 144) == -1);   // page 9 of 8
+  CHECK(look(0, 192) == -1);   // past the columns
+  CHECK(look(1, 48) == -1 && look(1, 96) == -1 && look(1, 144) == -1 && look(2, 0) == -1);
+  CHECK(look(2, 50) == 4 && look(2, -1) == -1);
+  CHECK(look(-1, 0) == -1 && look(3, 0) == -1 && look(int64_t(1) << 62, 0) == -1);
+  CHECK(look(0, int64_t(1) << 62) == -1 && look(0, -(int64_t(1) << 62)) == -1);
   CHECK(steps_of(-1) == 0 && steps_of(0) == 1 && steps_of(15) == 1 && steps_of(16) == 2);
 
   // even splits: the ranges tile [0, total), differ by one at most, and split_owner inverts them
