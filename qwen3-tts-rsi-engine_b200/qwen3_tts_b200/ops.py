@@ -529,57 +529,55 @@ def decode_attention_qkv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin_
 
 
 # ------------------------------------------------------------------ paged key/value cache
-# These wrappers are called once or twice per layer and token, so their checks read each attribute once and use the
-# cheap forms (get_device, identity of dtypes); the arguments travel as one packed struct.
+# These wrappers are called once or twice per layer and token, so each attribute is read once, in its cheap form
+# (get_device, identity of dtypes), and the arguments travel as one packed struct.
+_INT64, _INT32 = torch.int64, torch.int32
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 def _paged_cache(what: str, device: int, key_pages, value_pages, page_table):
-    """Check the pool and the page table; the leading fields of a packed call and the table's row count."""
+    """Check the pool and the page table; the leading fields of a packed call."""
     if (device < 0 or key_pages.get_device() != device or value_pages.get_device() != device
             or page_table.get_device() != device):
         raise ValueError(f"{what}: expected CUDA tensors on one device")
-    if key_pages.dtype is not BF16 or value_pages.dtype is not BF16 or key_pages.dim() != 4:
-        raise ValueError(f"{what}: expected BF16 key and value pages [pages, Hkv, page_size, D]")
-    pages, heads, size, dim = shape = key_pages.shape
-    stride = key_pages.stride()
-    if (value_pages.shape != shape or value_pages.stride() != stride or stride[3] != 1 or stride[2] != dim
-            or stride[1] != size * dim):
-        raise ValueError(f"{what}: pages must be dense [Hkv, page_size, D] blocks, keys and values laid out alike")
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2:
-        raise ValueError(f"{what}: page table must be INT32 [sequences, columns]")
-    rows, columns = page_table.shape
-    row_stride, inner = page_table.stride()
-    if inner != 1:
-        raise ValueError(f"{what}: page table rows must have unit stride")
-    return (key_pages.data_ptr(), value_pages.data_ptr(), stride[0], pages, size, heads, dim, page_table.data_ptr(),
-            row_stride, rows, columns, device)
+    shape, stride = key_pages.shape, key_pages.stride()
+    if (key_pages.dtype is not BF16 or value_pages.dtype is not BF16 or len(shape) != 4 or value_pages.shape != shape
+            or value_pages.stride() != stride):
+        raise ValueError(f"{what}: expected BF16 key and value pages [pages, Hkv, page_size, D], laid out alike")
+    pages, heads, size, dim = shape
+    page_stride, head_stride, row_stride, inner = stride
+    if inner != 1 or row_stride != dim or head_stride != size * dim:
+        raise ValueError(f"{what}: pages must be dense [Hkv, page_size, D] blocks")
+    shape, stride = page_table.shape, page_table.stride()
+    if page_table.dtype is not _INT32 or len(shape) != 2 or stride[1] != 1:
+        raise ValueError(f"{what}: page table must be INT32 [sequences, columns] with unit inner stride")
+    return (key_pages.data_ptr(), value_pages.data_ptr(), page_stride, pages, size, heads, dim, page_table.data_ptr(),
+            stride[0], shape[0], shape[1], device)
 
 
 def _paged_index(what: str, name: str, t, device: int, count: int) -> int:
-    if (t.get_device() != device or t.dtype is not torch.int64 or t.dim() != 1 or t.shape[0] != count
-            or not t.is_contiguous()):
+    if t.get_device() != device or t.dtype is not _INT64 or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous INT64 CUDA vector of {count}")
     return t.data_ptr()
 
 
-def _paged_query(what: str, query, dim: int, kv_heads: int, out):
+def _paged_query(what: str, query, dim: int, kv_heads: int, out, device: int):
     """(rows, query heads, row stride) of a query [rows, Hq, D] whose rows are dense."""
-    if query.dtype is not BF16 or query.dim() != 3:
-        raise ValueError(f"{what}: query must be BF16 [rows, Hq, D]")
-    rows, heads, width = shape = query.shape
-    stride = query.stride()
-    if width != dim or stride[2] != 1 or stride[1] != dim or heads % kv_heads:
-        raise ValueError(f"{what}: query rows must be dense [Hq, D], Hq a multiple of Hkv")
-    if out is not None and (out.shape != shape or out.dtype is not BF16 or not out.is_contiguous()
-                            or out.get_device() != query.get_device()):
+    shape, stride = query.shape, query.stride()
+    if (query.dtype is not BF16 or len(shape) != 3 or shape[2] != dim or stride[2] != 1 or stride[1] != dim
+            or shape[1] % kv_heads):
+        raise ValueError(f"{what}: query must be BF16 [rows, Hq, D] with dense rows, Hq a multiple of Hkv")
+    if out is not None and (out.get_device() != device or out.dtype is not BF16 or out.shape != shape
+                            or not out.is_contiguous()):
         raise ValueError(f"{what}: out must be contiguous BF16 shaped like query")
-    return rows, heads, stride[0]
+    return shape[0], shape[1], stride[0]
 
 
 def _paged_workspace(what: str, need: int, workspace, device: int):
     """(tensor, pointer, bytes): the caller's workspace, or one of this call's own, from the caching allocator of
     the current stream (inside a capture: of the graph). Calls and graphs never share one unasked."""
     if workspace is None:
-        if need == 0:
-            return None, 0, 0
         workspace = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", device))
     elif workspace.get_device() != device or not workspace.is_contiguous():
         raise ValueError(f"{what}: workspace must be a contiguous tensor on the query's device")
@@ -587,7 +585,9 @@ def _paged_workspace(what: str, need: int, workspace, device: int):
 
 
 def _paged_call(name: str, packed: bytes, device: int) -> None:
-    call(name, packed, SCRATCH.status_pointer(device), torch._C._cuda_getCurrentRawStream(device))
+    rc = getattr(_lib.load(), name)(packed, SCRATCH.status_pointer(device), _raw_stream(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def paged_qk_norm_rope_kv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin_table, rotary_positions,
@@ -603,12 +603,11 @@ def paged_qk_norm_rope_kv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin
     what = "paged_qk_norm_rope_kv"
     device = qkv.get_device()
     cache = _paged_cache(what, device, key_pages, value_pages, page_table)
-    if qkv.dtype is not BF16 or qkv.dim() != 2 or cache[5] != kv_heads or cache[6] != head_dim:
-        raise ValueError(f"{what}: qkv must be BF16 [rows, (q + 2 kv) * head_dim] for the pages' heads")
-    rows, width = qkv.shape
-    row_stride, inner = qkv.stride()
-    if width != (q_heads + 2 * kv_heads) * head_dim or inner != 1:
-        raise ValueError(f"{what}: qkv must be [rows, (q + 2 kv) * head_dim] with unit inner stride")
+    shape, stride = qkv.shape, qkv.stride()
+    if (qkv.dtype is not BF16 or len(shape) != 2 or shape[1] != (q_heads + 2 * kv_heads) * head_dim or stride[1] != 1
+            or cache[5] != kv_heads or cache[6] != head_dim):
+        raise ValueError(f"{what}: qkv must be BF16 [rows, (q + 2 kv) * head_dim], unit inner stride, for the pages' heads")
+    rows = shape[0]
     rotary = _paged_index(what, "rotary_positions", rotary_positions, device, rows)
     positions = _paged_index(what, "cache_positions", cache_positions, device, rows)
     if sequences is not None:
@@ -617,13 +616,13 @@ def paged_qk_norm_rope_kv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin
         raise ValueError(f"{what}: page table must have a row per qkv row")
     table_shape = cos_table.shape
     if (cos_table.dtype is not BF16 or sin_table.dtype is not BF16 or cos_table.get_device() != device
-            or sin_table.get_device() != device or cos_table.dim() != 2 or table_shape[1] != head_dim
+            or sin_table.get_device() != device or len(table_shape) != 2 or table_shape[1] != head_dim
             or sin_table.shape != table_shape or not cos_table.is_contiguous() or not sin_table.is_contiguous()):
         raise ValueError(f"{what}: cos and sin tables must be contiguous BF16 [positions, head_dim]")
     norms = 0, 0
     if q_norm_weight is not None or k_norm_weight is not None:
         for w in (q_norm_weight, k_norm_weight):
-            if (w is None or w.get_device() != device or w.dtype is not BF16 or w.numel() != head_dim
+            if (w is None or w.get_device() != device or w.dtype is not BF16 or w.shape != (head_dim,)
                     or not w.is_contiguous()):
                 raise ValueError(f"{what}: norm weights must both be contiguous BF16 [head_dim], or both None")
         norms = q_norm_weight.data_ptr(), k_norm_weight.data_ptr()
@@ -634,7 +633,7 @@ def paged_qk_norm_rope_kv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin
         raise ValueError(f"{what}: query_out must be contiguous BF16 [rows, q_heads, head_dim]")
     if rows:
         _paged_call("q3t_paged_qk_norm_rope_kv", _lib.PAGED_WRITE.pack(
-            *cache, qkv.data_ptr(), row_stride, rows, q_heads, *norms, cos_table.data_ptr(), sin_table.data_ptr(),
+            *cache, qkv.data_ptr(), stride[0], rows, q_heads, *norms, cos_table.data_ptr(), sin_table.data_ptr(),
             table_shape[0], rotary, positions, sequences or 0, query_out.data_ptr(), eps), device)
     return query_out
 
@@ -656,7 +655,7 @@ def paged_decode_attention(query, key_pages, value_pages, page_table, positions,
     device = query.get_device()
     cache = _paged_cache(what, device, key_pages, value_pages, page_table)
     _, _, _, _, size, kv_heads, dim, _, _, table_rows, columns, _ = cache
-    rows, q_heads, row_stride = _paged_query(what, query, dim, kv_heads, out)
+    rows, q_heads, row_stride = _paged_query(what, query, dim, kv_heads, out, device)
     at = _paged_index(what, "positions", positions, device, rows)
     if table_rows < rows:
         raise ValueError(f"{what}: page table must have a row per query row")
@@ -665,7 +664,7 @@ def paged_decode_attention(query, key_pages, value_pages, page_table, positions,
         out = torch.empty(query.shape, dtype=BF16, device=query.device)
     if rows:
         need = paged_decode_attention_workspace_bytes(rows, q_heads, kv_heads, dim, context)
-        held, ws, ws_bytes = _paged_workspace(what, need, workspace, device)
+        held, ws, ws_bytes = (None, 0, 0) if need == 0 else _paged_workspace(what, need, workspace, device)
         _paged_call("q3t_paged_decode_attention", _lib.PAGED_DECODE.pack(
             *cache, query.data_ptr(), row_stride, rows, q_heads, at, out.data_ptr(), context,
             dim ** -0.5 if scale is None else scale, ws, ws_bytes), device)
@@ -690,7 +689,7 @@ def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offse
     device = query.get_device()
     cache = _paged_cache(what, device, key_pages, value_pages, page_table)
     _, _, _, _, size, kv_heads, dim, _, _, table_rows, columns, _ = cache
-    rows, q_heads, row_stride = _paged_query(what, query, dim, kv_heads, out)
+    rows, q_heads, row_stride = _paged_query(what, query, dim, kv_heads, out, device)
     sequences = start_positions.numel()
     starts = _paged_index(what, "start_positions", start_positions, device, sequences)
     offsets = _paged_index(what, "row_offsets", row_offsets, device, sequences + 1)
@@ -698,7 +697,7 @@ def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offse
         raise ValueError(f"{what}: page table must have a row per sequence")
     if rows and sequences:
         need = paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, dim, columns * size)
-        held, ws, ws_bytes = _paged_workspace(what, need, workspace, device)
+        held, ws, ws_bytes = (None, 0, 0) if need == 0 else _paged_workspace(what, need, workspace, device)
         _paged_call("q3t_paged_prefill_attention", _lib.PAGED_PREFILL.pack(
             *cache, query.data_ptr(), row_stride, rows, q_heads, offsets, starts, sequences, out.data_ptr(),
             dim ** -0.5 if scale is None else scale, ws, ws_bytes), device)

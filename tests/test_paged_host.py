@@ -184,7 +184,7 @@ BAD = [(decode, c) for c in SHARED + [
     dict(query=torch.zeros(3, 4, 128, dtype=BF16)), dict(query=torch.zeros(3, 8, 64, dtype=BF16)[:, ::2]),
     dict(query=torch.zeros(3, 4, 128, dtype=BF16)[..., ::2]), dict(query=torch.zeros(4, 64, dtype=BF16)),
     dict(positions=index(2)), dict(positions=index(3, torch.int32)), dict(positions=index(6)[::2]),
-    dict(positions=index(3)[:, None]), dict(out=torch.zeros(3, 4, 64)), dict(out=torch.zeros(2, 4, 64, dtype=BF16)),
+    dict(positions=index(3)[:, None]), dict(positions=index(6)[::2]), dict(out=torch.zeros(3, 4, 64)), dict(out=torch.zeros(2, 4, 64, dtype=BF16)),
     dict(out=torch.zeros(6, 4, 64, dtype=BF16)[::2])]]
 BAD += [(prompt, c) for c in SHARED + [
     dict(offsets=index(3)), dict(offsets=index(4, torch.int32)), dict(starts=index(2)), dict(starts=index(6)[::2]),
