@@ -442,7 +442,6 @@ int launch_direct(DecodeArgs& a, const PromptRows& pr, int ranks, void* stream, 
 struct SplitArgs {
   int parts;      // CTAs = ranges
   int heads;      // query heads of a pass at most
-  int32_t* prefix;  // workspace: steps before row r, of one KV head and pass; [rows + 1]
   float* partial;   // workspace: [parts][2][heads][D + 2]: the item a range begins inside of (0) or ends inside of (1)
 };
 
@@ -526,8 +525,6 @@ __global__ void __launch_bounds__(W * 32, 1) paged_decode_split(const DecodeArgs
   if (threadIdx.x == 0) prefix[a.rows] = carry;
   if (threadIdx.x < 2 * W) resting[threadIdx.x].valid = 0;
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int r = threadIdx.x; r <= a.rows; r += kThreads) sp.prefix[r] = prefix[r];
   for (int r = blockIdx.x; r < a.rows; r += sp.parts)
     if (prefix[r] == prefix[r + 1])
       for (int e = threadIdx.x; e < a.q_heads * D / 8; e += kThreads)
@@ -662,40 +659,97 @@ __global__ void __launch_bounds__(W * 32, 1) paged_decode_split(const DecodeArgs
   }
 }
 
-// The items that several ranges share: one CTA joins their partial runs in the order of the ranges.
+// The items that several ranges share: one CTA joins their partial runs in the order of the ranges. It finds them from
+// the positions alone, before it waits for the launch that it depends on (that one has waited for everything before it),
+// and up to kAtOnce parts are read in one round of loads (3 rows of 20000..65535 keys: 84.3 -> 79.7 us in all). No CTA
+// leaves before the wait: what follows this launch may rely on its end for the end of both.
+constexpr int kJoinThreads = 256, kAtOnce = 8;
+
 template <int D>
-__global__ void __launch_bounds__(128) paged_decode_join(const DecodeArgs a, const SplitArgs sp) {
+__global__ void __launch_bounds__(kJoinThreads) paged_decode_join(const DecodeArgs a, const SplitArgs sp) {
   extern __shared__ float weight[];  // [heads][parts], then [heads] sums
-  grid_dependency_wait();
+  __shared__ int sums[2][kJoinThreads / 32];
   const int units = a.kv_heads * a.passes, row = int(blockIdx.x / units), unit = int(blockIdx.x % units);
-  const int64_t total = int64_t(sp.prefix[a.rows]) * units;
-  const int32_t n = sp.prefix[row + 1] - sp.prefix[row];
-  if (n == 0) return;
-  const int64_t begin = int64_t(sp.prefix[row]) * units + int64_t(unit) * n;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto steps = [&](int r) { return int(steps_of(min(a.positions[r], a.context - 1))); };
+  int before = 0, all = 0;
+  for (int r = threadIdx.x; r < a.rows; r += kJoinThreads) {
+    const int n = steps(r);
+    all += n;
+    before += r < row ? n : 0;
+  }
+  const int n = steps(row);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+  }
+  if (lane == 0) sums[0][warp] = all, sums[1][warp] = before;
+  __syncthreads();
+  all = before = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) all += sums[0][w], before += sums[1][w];
+  if (n == 0) {
+    grid_dependency_wait();
+    return;
+  }
+  const int64_t total = int64_t(all) * units, begin = int64_t(before) * units + int64_t(unit) * n;
   const int64_t ranges = split_parts(total, sp.parts);
   const int first = int(split_owner(begin, total, ranges)), last = int(split_owner(begin + n - 1, total, ranges));
-  if (first == last) return;
+  if (first == last) {
+    grid_dependency_wait();
+    return;
+  }
   const int pass = unit % a.passes, heads = min(kHeads, a.group - pass * kHeads), part = sp.heads * (D + 2);
   // ranges after the first begin inside the item
   const int slot = begin > split_begin(first, total, ranges);
   auto at = [&](int i) { return sp.partial + (int64_t(first + i) * 2 + (i == 0 ? slot : 0)) * part; };
-  const int count = last - first + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* sums = weight + sp.heads * sp.parts;
-  for (int h = warp; h < heads; h += 4) {
+  const int count = last - first + 1, head0 = unit / a.passes * a.group + pass * kHeads;
+  __nv_bfloat16* out = a.out + (int64_t(row) * a.q_heads + head0) * D;
+  grid_dependency_wait();
+  if (count <= kAtOnce) {
+    for (int e = threadIdx.x; e < heads * D / 2; e += kJoinThreads) {
+      const int h = e / (D / 2), d = e % (D / 2) * 2;
+      float2 ml[kAtOnce], o[kAtOnce];
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f), o[i] = make_float2(0.f, 0.f);
+        if (i < count) {
+          const float* p = at(i) + h * (D + 2);
+          ml[i] = *reinterpret_cast<const float2*>(p);
+          o[i] = *reinterpret_cast<const float2*>(p + 2 + d);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, ml[i].x);
+      float l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float f = ml[i].x == top ? 1.f : exp2_fast(ml[i].x - top);
+        l += ml[i].y * f;
+        o0 += o[i].x * f;
+        o1 += o[i].y * f;
+      }
+      *reinterpret_cast<uint32_t*>(out + h * D + d) = pack2(o0 / l, o1 / l);
+    }
+    return;
+  }
+  float* total_l = weight + sp.heads * sp.parts;
+  for (int h = warp; h < heads; h += kJoinThreads / 32) {
     float top = -INFINITY, l = 0.f;
     for (int i = lane; i < count; i += 32) top = fmaxf(top, at(i)[h * (D + 2)]);
     top = warp_max(top);
     for (int i = lane; i < count; i += 32) {
-      const float m = at(i)[h * (D + 2)], f = m == top ? 1.f : exp2f(m - top);
+      const float m = at(i)[h * (D + 2)], f = m == top ? 1.f : exp2_fast(m - top);
       weight[h * sp.parts + i] = f;
       l += at(i)[h * (D + 2) + 1] * f;
     }
     l = warp_sum(l);
-    if (lane == 0) sums[h] = l;
+    if (lane == 0) total_l[h] = l;
   }
   __syncthreads();
-  const int head0 = unit / a.passes * a.group + pass * kHeads;
-  for (int e = threadIdx.x; e < heads * D / 2; e += 128) {
+  for (int e = threadIdx.x; e < heads * D / 2; e += kJoinThreads) {
     const int h = e / (D / 2), d = e % (D / 2) * 2;
     float o0 = 0.f, o1 = 0.f;
 #pragma unroll 8
@@ -704,20 +758,19 @@ __global__ void __launch_bounds__(128) paged_decode_join(const DecodeArgs a, con
       o0 += v.x * weight[h * sp.parts + i];
       o1 += v.y * weight[h * sp.parts + i];
     }
-    *reinterpret_cast<uint32_t*>(a.out + (int64_t(row) * a.q_heads + head0 + h) * D + d) = pack2(o0 / sums[h], o1 / sums[h]);
+    *reinterpret_cast<uint32_t*>(out + h * D + d) = pack2(o0 / total_l[h], o1 / total_l[h]);
   }
 }
 
 struct SplitPlan {
   int parts, heads;
-  size_t prefix_bytes, bytes;
+  size_t bytes;
 };
-SplitPlan split_plan(int64_t rows, int64_t group, int64_t head_dim) {
+SplitPlan split_plan(int64_t group, int64_t head_dim) {
   SplitPlan p;
   p.parts = sm_count();
   p.heads = int(group < kHeads ? group : kHeads);
-  p.prefix_bytes = size_t((rows + 1) * 4 + 15) / 16 * 16;
-  p.bytes = p.prefix_bytes + size_t(p.parts) * 2 * p.heads * (head_dim + 2) * 4;
+  p.bytes = size_t(p.parts) * 2 * p.heads * (head_dim + 2) * 4;
   return p;
 }
 
@@ -752,13 +805,12 @@ int launch_split(const DecodeArgs& a, void* workspace, void* stream, const char*
   static PerDevice once;
   constexpr int kMost = 232448;
   if (const int rc = smem_limit(once, paged_decode_split<D, W, ST>, kMost, name)) return rc;
-  const SplitPlan p = split_plan(a.rows, a.group, D);
-  SplitArgs sp = {p.parts, p.heads, static_cast<int32_t*>(workspace),
-                  reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.prefix_bytes)};
+  const SplitPlan p = split_plan(a.group, D);
+  const SplitArgs sp = {p.parts, p.heads, static_cast<float*>(workspace)};
   if (const int rc = launch(paged_decode_split<D, W, ST>, dim3(unsigned(p.parts)), dim3(W * 32),
                             size_t(split_smem<D, W, ST>(p.heads, a.rows)), stream, true, name, a, sp))
     return rc;
-  return launch(paged_decode_join<D>, dim3(unsigned(int64_t(a.rows) * a.kv_heads * a.passes)), dim3(128),
+  return launch(paged_decode_join<D>, dim3(unsigned(int64_t(a.rows) * a.kv_heads * a.passes)), dim3(kJoinThreads),
                 size_t(p.heads) * (p.parts + 1) * 4, stream, true, name, a, sp);
 }
 
@@ -796,7 +848,7 @@ extern "C" size_t q3t_paged_decode_attention_workspace_bytes(int64_t rows, int64
                                                              int64_t head_dim, int64_t context) {
   if (rows < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 1 || !decode_plan(rows, q_heads, kv_heads, context).split)
     return 0;
-  return split_plan(rows, q_heads / kv_heads, head_dim).bytes;
+  return split_plan(q_heads / kv_heads, head_dim).bytes;
 }
 
 extern "C" int q3t_paged_decode_attention(const q3t_paged_decode* call, unsigned* status, void* stream) {
@@ -815,7 +867,7 @@ extern "C" int q3t_paged_decode_attention(const q3t_paged_decode* call, unsigned
   const DecodePlan how = decode_plan(p.rows, p.q_heads, p.cache.kv_heads, p.context);
   const bool d128 = p.cache.head_dim == 128;
   if (how.split) {
-    const SplitPlan plan = split_plan(p.rows, a.group, p.cache.head_dim);
+    const SplitPlan plan = split_plan(a.group, p.cache.head_dim);
     if (p.workspace == nullptr || p.workspace_bytes < int64_t(plan.bytes) || !aligned16(p.workspace))
       return fail(Q3T_ESPACE, "%s: workspace of %zu bytes (16-byte aligned) needed", name, plan.bytes);
     return d128 ? launch_split<128, 8, 2>(a, p.workspace, stream, name)

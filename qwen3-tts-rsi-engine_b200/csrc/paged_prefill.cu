@@ -817,36 +817,40 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of an item that several ranges share: CTA (i, quarter) the 64 rows of the item that range i began and
-// did not end.
+// Joins the parts of an item that several ranges share: CTA (i, eighth) the 32 rows of the item that range i began and
+// did not end. Its parts are slot 1 of range i and slot 0 of the ranges after it, up to the item's end.
 template <int D>
 __global__ void __launch_bounds__(256) paged_prefill_join(const PrefillArgs a) {
   grid_dependency_wait();
-  const Segment first = a.shared_segments[blockIdx.x * 2 + 1];
+  const int lane = threadIdx.x & 31;
+  const Segment* segments = a.shared_segments + blockIdx.x * 2 + 1;
+  const Segment first = segments[0];
   if (first.count == 0) return;
-  const int row = blockIdx.y * 64 + (threadIdx.x & 63), chunk0 = (threadIdx.x >> 6) * (D / 16);  // of D / 4
-  const int t = row >> 7, p = (row & 127) / a.heads, h = (row & 127) % a.heads;
+  int parts = 1;
+  for (int base = 1; first.key_tiles < first.all_tiles; base += 32) {  // 32 ranges at a time
+    const bool there = int(blockIdx.x) + base + lane < a.parts;
+    const bool last = !there || segments[2 * (base + lane) - 1].tile0 + segments[2 * (base + lane) - 1].key_tiles >= first.all_tiles;
+    const unsigned hit = __ballot_sync(0xffffffffu, last);
+    parts = base + (hit ? __ffs(hit) : 32);
+    if (hit) break;
+  }
+  parts = min(parts, a.parts - int(blockIdx.x));
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), chunk0 = (threadIdx.x >> 5) * (D / 32);  // of D / 4
+  const int t = row >> 7, p = (row & 127) / a.heads, h = (row & 127) - p * a.heads;
   const int count = max(0, min(a.positions, first.count - t * a.positions));
   if (p >= count || h >= first.heads) return;
-  // parts: slot 1 of this range, then slot 0 of the next ones up to the item's end
   auto part_of = [&](int i) { return a.partial + (int64_t(blockIdx.x + i) * 2 + (i == 0)) * kPartFloats<D>; };
   float top = -INFINITY;
-  int parts = 0;
-  for (int end = first.key_tiles;; ++parts) {
-    top = fmaxf(top, part_of(parts)[256 * D + 2 * row]);
-    if (end >= first.all_tiles || int(blockIdx.x) + parts + 1 >= a.parts) break;
-    const Segment& next = a.shared_segments[(blockIdx.x + parts + 1) * 2];
-    end = next.tile0 + next.key_tiles;
-  }
-  ++parts;
-  float l = 0.f, v[D / 4] = {};
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) top = fmaxf(top, part_of(i)[256 * D + 2 * row]);
+  float l = 0.f, v[D / 8] = {};
   for (int i = 0; i < parts; ++i) {
     const float* part = part_of(i);
     const float2 ml = *reinterpret_cast<const float2*>(part + 256 * D + 2 * row);
     const float f = ml.x == top ? 1.f : exp2_fast(ml.x - top);
     l += ml.y * f;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
+    for (int c = 0; c < D / 32; ++c) {
       const float4 o = *reinterpret_cast<const float4*>(part + ((chunk0 + c) * 256 + row) * 4);
       v[4 * c] += o.x * f;
       v[4 * c + 1] += o.y * f;
@@ -858,7 +862,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join(const PrefillArgs a) {
   const float inv = top == INFINITY ? NAN : 1.f / l;
   __nv_bfloat16* out = a.out + (int64_t(first.row + t * a.positions + p) * a.q_heads + first.head0 + h) * D + chunk0 * 4;
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
+  for (int c = 0; c < D / 64; ++c) {
     float w[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = none ? 0.f : v[8 * c + e] * inv;
@@ -884,7 +888,7 @@ int launch_prefill(const q3t_paged_prefill& p, const PrefillArgs& a, int64_t blo
                             true, name, tmq, tmk, tmv, a))
     return rc;
   if (a.parts == 0) return Q3T_OK;
-  return launch(paged_prefill_join<D>, dim3(unsigned(a.parts), 4), dim3(256), 0, stream, true, name, a);
+  return launch(paged_prefill_join<D>, dim3(unsigned(a.parts), 8), dim3(256), 0, stream, true, name, a);
 }
 
 // How a call runs, from sizes that the host knows.
