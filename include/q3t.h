@@ -378,8 +378,8 @@ int q3t_decode_attention_noalloc(const void* query, const void* keys, const void
  * (SlotArena, continuous.py:97-132): every slot owns the longest context's rows, and growing copies
  * them all. Here sequences share a pool of pages. key_pages / value_pages: bf16 [pages, kv_heads,
  * page_size, head_dim], page stride in elements (both pools the same; a multiple of 8), everything
- * below it dense; page_size a multiple of 16; head_dim 64 or 128. page_table: int32 [sequences,
- * columns] (row stride table_stride), row s the pages of sequence s in order: position p is row
+ * below it dense; page_size a multiple of 16 up to 65536; head_dim 64 or 128. page_table: int32 [sequences,
+ * columns] (row stride table_stride; columns * page_size up to 2^34), row s the pages of sequence s in order: position p is row
  * p % page_size of page page_table[s][p / page_size]. Entries past a sequence's last position are not
  * read. A page may be shared by sequences that read it. Where the table has no valid page for a
  * position that a call needs, nothing out of range is touched and the status word's bad-index bit is

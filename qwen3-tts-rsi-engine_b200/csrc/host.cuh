@@ -88,6 +88,8 @@ inline int check_cache(const char* name, const q3t_paged_cache& c) {
   if (c.table_rows < 1 || c.table_columns < 1 || c.table_columns > 2147483647 ||
       (c.table_rows > 1 && c.table_stride < c.table_columns))
     return fail(Q3T_EINVAL, "%s: invalid page table", name);
+  if (c.table_columns > (int64_t(1) << 34) / c.page_size)  // steps of 16 keys are counted in 32 bits
+    return fail(Q3T_EUNSUPPORTED, "%s: table_columns * page_size beyond 2^34", name);
   if (((reinterpret_cast<uintptr_t>(c.key_pages) | reinterpret_cast<uintptr_t>(c.value_pages)) & 15u) != 0)
     return fail(Q3T_EINVAL, "%s: 16-byte alignment", name);
   return Q3T_OK;

@@ -667,7 +667,7 @@ def paged_decode_attention(query, key_pages, value_pages, page_table, positions,
         held, ws, ws_bytes = (None, 0, 0) if need == 0 else _paged_workspace(what, need, workspace, device)
         _paged_call("q3t_paged_decode_attention", _lib.PAGED_DECODE.pack(
             *cache, query.data_ptr(), row_stride, rows, q_heads, at, out.data_ptr(), context,
-            dim ** -0.5 if scale is None else scale, ws, ws_bytes), device)
+            dim ** -0.5 if scale is None else float(scale), ws, ws_bytes), device)
     return out
 
 
@@ -683,8 +683,8 @@ def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offse
 
     Sequence s owns query rows row_offsets[s] .. row_offsets[s + 1] - 1; its i-th row has position
     start_positions[s] + i (start > 0: a chunk after a cached prefix; negative positions are left padding and
-    give zeros) and sees keys 0 .. that position in the pages of page_table[s], which hold them already. Rows
-    that no sequence owns are left as they are in `out`. `workspace`: as for paged_decode_attention."""
+    give zeros) and sees keys 0 .. that position in the pages of page_table[s], which hold them already and finite.
+    Rows that no sequence owns are left as they are in `out`, which must not overlap query or pages. `workspace`: as for paged_decode_attention."""
     what = "paged_prefill_attention"
     device = query.get_device()
     cache = _paged_cache(what, device, key_pages, value_pages, page_table)
@@ -700,7 +700,7 @@ def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offse
         held, ws, ws_bytes = (None, 0, 0) if need == 0 else _paged_workspace(what, need, workspace, device)
         _paged_call("q3t_paged_prefill_attention", _lib.PAGED_PREFILL.pack(
             *cache, query.data_ptr(), row_stride, rows, q_heads, offsets, starts, sequences, out.data_ptr(),
-            dim ** -0.5 if scale is None else scale, ws, ws_bytes), device)
+            dim ** -0.5 if scale is None else float(scale), ws, ws_bytes), device)
     return out
 
 

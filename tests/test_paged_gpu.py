@@ -491,6 +491,112 @@ def test_a_workspace_of_the_caller(ops, cuda):
         ops.paged_decode_attention(query, keys, values, table, at, workspace=held.cpu())
 
 
+@pytest.mark.parametrize("capacity", [512, 1 << 17], ids=["in-turn", "ranges"])
+def test_prompts_repeat_bit_for_bit_captured_and_on_another_stream(ops, cuda, capacity):
+    """Eager, replayed and on a second stream at once: the same bits, whichever CTA took which item."""
+    counts, starts = [300, 1, 170, 90] * 5, [0, 200, 37, 0] * 5
+    made = []
+    for seed in range(2):
+        case = Case([n + s for n, s in zip(counts, starts)], 8, 128, 64, seed=seed, columns=capacity // 64)
+        query = rows_of((sum(counts), 16, 128), 30 + seed, False).to(cuda)
+        offsets = torch.tensor([sum(counts[:i]) for i in range(len(counts) + 1)], device=cuda)
+        args = (query, *case.to(cuda), offsets, torch.tensor(starts, device=cuda))
+        made.append((args, ops.paged_prefill_attention(*args, out=torch.zeros_like(query))))
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(made[0][1])
+    with torch.cuda.graph(graph):
+        ops.paged_prefill_attention(*made[0][0], out=out)
+    side, other = torch.cuda.Stream(), torch.zeros_like(made[1][1])
+    torch.cuda.synchronize()
+    for _ in range(10):
+        out.zero_(), other.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            ops.paged_prefill_attention(*made[1][0], out=other)
+        torch.cuda.synchronize()
+        assert torch.equal(out, made[0][1]) and torch.equal(other, made[1][1])
+    assert ops.read_status(cuda) == 0
+
+
+def test_offsets_past_32_bits(ops, cuda):
+    """Pages whose elements lie past 2^31: the write, and both attentions."""
+    pages, kv, size, d = 40000, 8, 64, 128          # 2.6e9 elements a pool
+    keys, values = (torch.empty(pages, kv, size, d, dtype=BF16, device=cuda) for _ in range(2))
+    small = Case([130, 40], kv, d, size, seed=3)
+    k, v, table = small.to(cuda)
+    high = table.clone()
+    for s, n in ((0, 3), (1, 1)):
+        for j in range(n):
+            high[s, j] = pages - 1 - int(table[s, j])
+            keys[high[s, j]], values[high[s, j]] = k[table[s, j]], v[table[s, j]]
+    query = rows_of((2, 16, d), 1, False).to(cuda)
+    at = torch.tensor([129, 39], device=cuda)
+    assert torch.equal(ops.paged_decode_attention(query, keys, values, high, at),
+                       ops.paged_decode_attention(query, k, v, table, at))
+    prompt = rows_of((170, 16, d), 2, False).to(cuda)
+    offsets, starts = torch.tensor([0, 130, 170], device=cuda), torch.zeros(2, dtype=torch.int64, device=cuda)
+    assert torch.equal(ops.paged_prefill_attention(prompt, keys, values, high, offsets, starts, out=torch.zeros_like(prompt)),
+                       ops.paged_prefill_attention(prompt, k, v, table, offsets, starts, out=torch.zeros_like(prompt)))
+    cos, sin = (t.to(cuda) for t in tables(140, d))
+    qkv = rows_of((2, 32 * d), 4, False).to(cuda)
+    for pool in ((k, v, table), (keys, values, high)):
+        ops.paged_qk_norm_rope_kv(qkv, None, None, 1e-6, cos, sin, at, at, pool[2], pool[0], pool[1], q_heads=16,
+                                  kv_heads=8, head_dim=d)
+    assert torch.equal(keys[high[0, 2], :, 1], k[table[0, 2], :, 1])
+    assert torch.equal(values[high[1, 0], :, 39], v[table[1, 0], :, 39])
+    assert ops.read_status(cuda) == 0
+
+
+def test_misaligned_tensors_are_refused(ops, cuda):
+    case = Case([20], 2, 64, 16)
+    keys, values, table = case.to(cuda)
+    odd = torch.zeros(4 * 64 + 1, dtype=BF16, device=cuda)[1:].view(1, 4, 64)
+    with pytest.raises(ValueError, match="alignment"):
+        ops.paged_decode_attention(odd, keys, values, table, torch.tensor([19], device=cuda))
+    out = torch.empty(1, 4, 64, dtype=BF16, device=cuda)
+    with pytest.raises(ValueError, match="alignment"):
+        ops.paged_prefill_attention(odd, keys, values, table, torch.tensor([0, 1], device=cuda),
+                                    torch.tensor([19], device=cuda), out=out)
+    strided = torch.zeros(2, 4 * 64 + 4, dtype=BF16, device=cuda)[:, :256].unflatten(1, (4, 64))
+    with pytest.raises(ValueError, match="stride"):
+        ops.paged_decode_attention(strided, keys, values, table.repeat(2, 1), torch.tensor([19, 19], device=cuda))
+
+
+def test_an_output_that_is_only_16_byte_aligned(ops, cuda):
+    case = Case([150], 2, 64, 16)
+    keys, values, table = case.to(cuda)
+    query = rows_of((150, 4, 64), 5, False).to(cuda)
+    offsets, starts = torch.tensor([0, 150], device=cuda), torch.zeros(1, dtype=torch.int64, device=cuda)
+    want = ops.paged_prefill_attention(query, keys, values, table, offsets, starts, out=torch.zeros_like(query))
+    out = torch.zeros(150 * 256 + 8, dtype=BF16, device=cuda)[8:].view(150, 4, 64)
+    assert torch.equal(ops.paged_prefill_attention(query, keys, values, table, offsets, starts, out=out), want)
+
+
+def test_prompts_with_odd_offsets_are_flagged(ops, cuda):
+    """Row offsets that leave the query or run backwards: that sequence is skipped, the others are right (where a row is
+    of two of them, each of its elements is one's or the other's)."""
+    case = Case([40, 40, 40], 8, 128, 16)
+    query = rows_of((120, 16, 128), 1, False)
+    keys, values, table = case.to(cuda)
+    starts = torch.zeros(3, dtype=torch.int64, device=cuda)
+    for offsets in ([0, 40, 80, 121], [-1, 40, 80, 120], [0, 40, 20, 60]):
+        for columns in (3, 3000):
+            wide = torch.full((3, columns), -1, dtype=torch.int32, device=cuda)
+            wide[:, :3] = table
+            out = torch.full_like(query, 5.0, device=cuda)
+            ops.paged_prefill_attention(query.to(cuda), keys, values, wide, torch.tensor(offsets, device=cuda), starts,
+                                        out=out)
+            assert ops.read_status(cuda) == 8
+            owners = [s for s in range(3) if 0 <= offsets[s] < offsets[s + 1] <= 120]
+            for r in range(120):
+                got, near, owned = out[r].double().cpu(), torch.zeros(16, 128, dtype=torch.bool), False
+                for s in owners:
+                    if offsets[s] <= r < offsets[s + 1]:
+                        want, bound = attend(query[r], *case.sequence(s, r - offsets[s] + 1), 128 ** -0.5)
+                        near, owned = near | ((got - want).abs() <= bound), True
+                assert near.all() if owned else (got == 5).all(), f"{offsets} row {r}"
+
+
 def test_empty_batches_and_given_outputs(ops, cuda):
     case = Case([20], 2, 64, 16)
     keys, values, table = case.to(cuda)

@@ -245,7 +245,8 @@ POOLS = [(dict(keys=None), -1), (dict(values=A16 + 2), -1), (dict(page_stride=20
          (dict(pages=0), -1), (dict(pages=1 << 31), -1), (dict(page_size=24), -2), (dict(page_size=0), -2),
          (dict(page_size=1 << 20), -2), (dict(kv=0), -1), (dict(dim=96), -2), (dict(table=None), -1),
          (dict(columns=0), -1), (dict(table_stride=1), -1), (dict(rows=0), -1),
-         (dict(table_rows=0), -1), (dict(table_rows=2), -1)]
+         (dict(table_rows=0), -1), (dict(table_rows=2), -1),
+         (dict(columns=(1 << 30) + 1, table_stride=1 << 31), -2)]
 C_BAD = [(c_decode, c, rc) for c, rc in POOLS + [
     (dict(query_stride=255), -1), (dict(query_stride=260), -1), (dict(q=5), -1), (dict(query=A16 + 8), -1),
     (dict(context=33), -1), (dict(context=0), -1), (dict(positions=None), -1), (dict(rows=1 << 31), -1)]]
