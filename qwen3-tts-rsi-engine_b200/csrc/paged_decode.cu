@@ -15,7 +15,7 @@
 //
 // A step's keys of one head are 16 adjacent rows of a page, and so are its values: each cp.async instruction
 // of a warp copies 512 adjacent bytes. (Copying instead what each lane will read back itself, 64-byte
-// pieces of 8 rows, needs neither swizzle nor warp barrier, but ran at 5.0 TB/s instead of 6.5: the memory
+// pieces of 8 rows, needs neither swizzle nor warp barrier, but ran at 5.0 TB/s instead of 6.7: the memory
 // system takes one request per 128-byte line an instruction touches.) The 16-byte chunks of a row are
 // permuted on their way so that no read has a bank conflict. With g = lane / 4, t = lane % 4 a lane reads
 //   K: keys g and g + 8 at dim chunks t, t + 4, ... (8 dims each); chunk c of key k is at c ^ 4 (k % 2).
@@ -267,9 +267,11 @@ Q3T_DEV void rest(const Run<D>& run, float* part, int heads, int g, int t) {
   }
 }
 
-// One CTA per (row, key/value head, pass), or a cluster of `ranks`: the warps share the row's steps in contiguous
-// runs, merge through shared memory, and a cluster's CTAs through distributed shared memory. PROMPT: row r is a packed prompt row, whose sequence and position follow from
-// row_offsets and start_positions.
+// One CTA per (row, key/value head, pass), or a cluster of `ranks`: the warps share the row's steps in contiguous runs,
+// merge through shared memory, and a cluster's CTAs through distributed shared memory. 256 rows of 1..4096 keys, 16 query
+// and 8 KV heads of 128 dims: 313 us for 2.17 GB, 6.9 TB/s (a plain read of memory reaches 7.1).
+// PROMPT: row r is a packed prompt row, whose sequence and position follow from row_offsets and start_positions; this is
+// the form of the prompt attention for what its tiled kernel does not take.
 struct PromptRows {
   const int64_t *row_offsets, *start_positions;
   int sequences;
@@ -783,7 +785,7 @@ SplitPlan split_plan(int64_t group, int64_t head_dim) {
 //   warps; 64 rows of 64..2048: 52, as good);
 // - contexts that would keep one CTA busy for long: the split kernel. With equal lengths the two are even (64 rows of
 //   4000..8192: 254 us split, 257 direct; 256 rows of 1..4096: 329 and 313), but one row of 8192 keys among 63 of 200
-//   takes 80 us direct and 28 split, one of 32768 among 7 takes 83 and 37.
+//   takes 80 us direct and 25 split, one of 32768 among 7 takes 83 and 36.
 struct DecodePlan {
   bool split;
   int ranks;   // direct: CTAs per item

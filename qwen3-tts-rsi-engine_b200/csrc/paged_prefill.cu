@@ -15,6 +15,10 @@
 // row's maximum exceeds by at most 8 (powers of two), so O in TMEM is rescaled only when a maximum moves by more; O / l
 // does not depend on it. P's rounding to bf16 is that of a bf16 tensor product; S, m, l and O stay in fp32.
 //
+// One prompt of 8191 rows with 32 query and 8 KV heads of 128 dims: 440 us, 1250 TFLOP/s (512 us over seconds, under the
+// power cap). A pair of 128 x 128 key tiles takes 3150 cycles of which the tensor cores work 2080: scores, the first half of
+// the weights, their product and the next scores wait for one another, and there is no TMEM for a third tile.
+//
 // Work comes in one of two ways (the host picks by sizes):
 // - items (query tile pair, KV head) in turn: a CTA whose item's loads are out takes over one that has not been launched
 //   yet, so items go to the SMs as those get free, and the next one's loads and first products overlap the last one's

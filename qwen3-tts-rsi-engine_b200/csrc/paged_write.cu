@@ -10,6 +10,11 @@
 // holds 8 dims of the first half and the 8 dims that rotate with them in the second, so RoPE needs no
 // exchange between lanes and the norm only the D/16-lane sum. A lane takes HEADS heads of a row, whose loads
 // are all on their way before the first is used, and reads the row's positions, cos and sin once for them.
+//
+// 3500 rows of 16 + 2 * 8 heads of 128 dims: 17.2 us for 65.8 MB, 3.8 TB/s; 16000 rows 4.8 TB/s; 1 to 64 rows 2.5 us. The
+// same kernel that only copies takes 11 us for the 3500: what is between is the chain of positions, cos/sin and the head's
+// sum in each thread, with as many threads as the registers allow. Fewer registers (a launch bound), two or eight heads to
+// a lane, packed fp32 arithmetic, and rows brought into shared memory by a copying warp were all slower.
 #include "common.cuh"
 #include "host.cuh"
 #include "paged.cuh"
