@@ -831,6 +831,7 @@ int fill(DecodeArgs& a, const char* name, const q3t_paged_cache& c, const void* 
   a.page_stride = c.page_stride;
   a.pages = PageTable{c.page_table, c.table_stride, c.table_rows, c.table_columns, c.pages, int(c.page_size)};
   a.positions = nullptr;
+  a.ranks = 1;
   a.out = static_cast<__nv_bfloat16*>(out);
   a.rows = int(rows);
   a.q_heads = int(q_heads);

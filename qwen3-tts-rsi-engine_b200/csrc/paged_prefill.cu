@@ -54,7 +54,6 @@ struct PrefillArgs {
   int piece;    // rows of a TMA box: gcd(page_size, 128)
   int capacity; // positions that a page table row can hold
   bool out_32;  // out is 32-byte aligned
-  int items;    // at most
   int parts;    // ranges, one per CTA; 0: whole items in turn
   struct Segment* shared_segments;  // workspace: [parts][2], what a range left unfinished at its start (0) and end (1)
   float* partial;                   // workspace: [parts][2][D / 4][256 rows][4], then [256][2] (m, l)
@@ -282,11 +281,18 @@ Q3T_DEV int keys_of(const PrefillArgs& a, int64_t end) { return end < 0 ? 0 : in
 Q3T_DEV int key_tiles_of(const PrefillArgs& a, int64_t end) { return (keys_of(a, end) + kTileKeys - 1) / kTileKeys; }
 
 // Query tile pairs are numbered from the last of the last sequence backwards, so that those with the most keys
-// come first. One warp finds the sequence, rows and key tiles of number `index`; count 0: there is none.
-Q3T_DEV Segment find_tile(const PrefillArgs& a, int index, int unit, int lane) {
+// come first. One warp finds the sequence, rows and key tiles of number `index`; count 0: there is none. `before`: where the
+// CTA has it, the numbers of the sequences behind each, the last one first; without it 32 sequences are looked at at once.
+Q3T_DEV Segment find_tile(const PrefillArgs& a, const int32_t* before, int index, int unit, int lane) {
   const int span = 2 * a.positions;
   Segment t = {};
-  for (int base = a.sequences - 1; base >= 0; base -= 32) {
+  int base = a.sequences - 1;
+  if (before != nullptr) {
+    const int i = row_of(before, a.sequences, index, 1);
+    base -= i;
+    index -= before[i];
+  }
+  for (; base >= 0; base -= 32) {
     const int s = base - lane;
     int n = 0, first = 0, tiles = 0;
     int64_t start = 0;
@@ -303,6 +309,7 @@ Q3T_DEV Segment find_tile(const PrefillArgs& a, int index, int unit, int lane) {
     }
     const unsigned hit = __ballot_sync(0xffffffffu, sum > index);
     if (hit == 0) {
+      if (before != nullptr) break;
       index -= __shfl_sync(0xffffffffu, sum, 31);
       continue;
     }
@@ -397,15 +404,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->done, 1);
       fence_mbar_init();
     }
-    __syncwarp();
-    if (a.parts == 0) {  // the CTA's only item
-      const Segment seg = find_tile(a, int(blockIdx.x) / units, int(blockIdx.x) % units, lane);
-      if (lane == 0 && seg.count > 0) {
-        bars->segments[0] = seg;
-        mbar_arrive(&bars->segment_full[0]);
-      }
-      given = seg.count > 0;
-    }
   } else if (warp == 2) {
     tmem_alloc(&bars->tmem, 512);
     tmem_relinquish();
@@ -414,11 +412,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tmk);
     prefetch_tmap(&tmv);
   }
-  // ---- the plan: work before every query tile pair, for one unit
+  // ---- the plan: the numbers behind every sequence, where it takes more than a look to find one; for ranges, the work
+  // before every query tile pair, for one unit
   int32_t* prefix = reinterpret_cast<int32_t*>(smem + M::kPlan);
+  int32_t* before = nullptr;
   int pairs = 0;
-  if (a.parts > 0) {
-    int32_t* before = prefix + kPlanTiles + 1;  // pairs of the sequences after s: numbers begin at the last one
+  if (a.parts > 0 || (a.sequences > 32 && a.sequences <= kPlanTiles)) {
+    before = a.parts > 0 ? prefix + kPlanTiles + 1 : prefix;
     const int span = 2 * a.positions;
     for (int s0 = 0; s0 < a.sequences; s0 += kThreads) {
       const int s = a.sequences - 1 - s0 - int(threadIdx.x);
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     int work = 0;
-    for (int e0 = 0; e0 < pairs; e0 += kThreads) {
+    for (int e0 = 0; a.parts > 0 && e0 < pairs; e0 += kThreads) {
       const int e = e0 + int(threadIdx.x);
       int cost = 0, all;
       if (e < pairs) {
@@ -443,7 +443,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (e < pairs) prefix[e] = work + sum - cost;
       work += all;
     }
-    if (threadIdx.x == 0) prefix[pairs] = work;
+    if (a.parts > 0 && threadIdx.x == 0) prefix[pairs] = work;
+  }
+  if (a.parts == 0 && warp == 3) {  // the CTA's first item
+    const Segment seg = find_tile(a, before, int(blockIdx.x) / units, int(blockIdx.x) % units, lane);
+    if (lane == 0 && seg.count > 0) {
+      bars->segments[0] = seg;
+      mbar_arrive(&bars->segment_full[0]);
+    }
+    given = seg.count > 0;
   }
   tc_fence_before();
   __syncthreads();
@@ -781,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = warp_wait(&bars->takeover, i, a.status, kStatusFlagTimeout);
           int block = 0;
           if (!ok || !taken_over(&bars->response, block)) break;
-          seg = find_tile(a, block / units, block % units, lane);
+          seg = find_tile(a, before, block / units, block % units, lane);
           if (seg.count > 0) {
             give(seg);
             ++items;
@@ -798,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t base = int64_t(prefix[e]) * units;
           const int unit = int((f - base) / n);
           const int64_t item = base + int64_t(unit) * n, end = item + n < f1 ? item + n : f1;
-          seg = find_tile(a, e, unit, lane);
+          seg = find_tile(a, before, e, unit, lane);
           seg.tile0 = f > item ? int(f - item) - kFixed : 0;
           seg.key_tiles = int(end - item) - kFixed - seg.tile0;
           seg.slot = f > item ? 0 : end < item + n ? 1 : -1;
@@ -960,7 +968,6 @@ int launch_prefill_tiles(const q3t_paged_prefill& p, unsigned* status, void* str
   a.scale_log2 = float(p.scale) * kLog2e;
   a.status = status;
   a.out_32 = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
-  a.items = int(plan.items);
   a.parts = plan.parts;
   a.shared_segments = static_cast<Segment*>(p.workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + size_t(plan.parts) * 2 * sizeof(Segment));

@@ -78,6 +78,11 @@ def test_write_pages_strides_and_rows_without_norm(ops, cuda, page, norm, stride
                 one_pool=one_pool)
 
 
+@pytest.mark.parametrize("q,kv,d,norm", [(16, 8, 128, True), (8, 8, 64, False), (14, 2, 64, True), (9, 1, 128, True)])
+def test_write_many_rows(ops, cuda, q, kv, d, norm):
+    check_write(ops, cuda, q, kv, d, 64, [1001, 3, 900], new=False, norm=norm, strided=True)
+
+
 @pytest.mark.parametrize("count", [1, 2, 64, 257])
 def test_write_step_batches(ops, cuda, count):
     check_write(ops, cuda, 16, 8, 128, 16, [1 + 7 * i % 60 for i in range(count)], new=True, norm=True, strided=False,
@@ -327,8 +332,19 @@ def test_prompt_wide_groups(ops, cuda):
     check_prompt(ops, cuda, 70, 1, 64, 16, [5, 40], [0, 3], columns=1000)
 
 
-def test_prompt_many_sequences(ops, cuda):
-    check_prompt(ops, cuda, 4, 2, 128, 16, [(7 * i) % 4 for i in range(1500)], [(5 * i) % 23 for i in range(1500)])
+@pytest.mark.parametrize("count", [31, 32, 33, 1024, 1500, 2048, 2049])
+def test_prompt_many_sequences(ops, cuda, count):
+    counts, starts = [(7 * i) % 4 for i in range(count)], [(5 * i) % 23 for i in range(count)]
+    check_prompt(ops, cuda, 4, 2, 128, 16, counts, starts)
+    if count <= 33:
+        check_prompt(ops, cuda, 4, 2, 128, 16, [5 * n for n in counts], [90 * n for n in starts], columns=1 << 13)
+
+
+def test_prompt_sequences_of_many_lengths(ops, cuda):
+    """Lengths around every multiple of a tile pair's positions, in an order that puts them at every offset."""
+    counts = [n + d for n in (128, 256, 384) for d in (-1, 0, 1)] + [1] * 40 + [127, 129, 255]
+    check_prompt(ops, cuda, 4, 2, 64, 16, counts, [0] * len(counts))
+    check_prompt(ops, cuda, 4, 2, 64, 16, counts[::-1], [0] * len(counts), columns=1 << 13, lead=3)
     check_prompt(ops, cuda, 4, 2, 128, 16, [(13 * i) % 41 for i in range(120)], [(5 * i) % 23 for i in range(120)])
 
 
