@@ -38,6 +38,13 @@ struct PageTable {
   }
 };
 
+// Where a packed sequence starts, kept far from the ends of 64 bits: its i-th row (i < 2^31) is at the result + i, which
+// is negative or past every table where the given position + i is, or would not be a number.
+Q3T_HD int64_t clamped_start(int64_t start) {
+  const int64_t most = int64_t(1) << 40;
+  return start > most ? most : start < -most ? -most : start;
+}
+
 // Decode attention streams keys in steps of 16, which never cross a page.
 constexpr int kStepKeys = 16;
 

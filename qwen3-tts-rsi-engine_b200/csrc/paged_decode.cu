@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
     }
     if (row < pr.row_offsets[lo] || row >= pr.row_offsets[lo + 1]) return;  // a row of no sequence
     sequence = lo;
-    position = pr.start_positions[lo] + (row - pr.row_offsets[lo]);
+    position = clamped_start(pr.start_positions[lo]) + (row - pr.row_offsets[lo]);
     if (position < 0) position = -1;
   } else {
     position = a.positions[row];

@@ -43,6 +43,7 @@ constexpr int kLeast = 4;          // key tiles of a part
 constexpr int kFixed = 2;          // what an item costs beside its key tiles, in key tiles
 constexpr int kPlanTiles = 2048;   // query tile pairs and sequences that a range plan holds
 constexpr int kPlanSequences = 1024;
+constexpr int kPlanPairs = 1 << 22;  // kThreads times as many are counted in 32 bits
 
 struct PrefillArgs {
   PageTable pages;
@@ -55,6 +56,7 @@ struct PrefillArgs {
   int capacity; // positions that a page table row can hold
   bool out_32;  // out is 32-byte aligned
   int parts;    // ranges, one per CTA; 0: whole items in turn
+  int pairs;    // query tile pairs at most
   struct Segment* shared_segments;  // workspace: [parts][2], what a range left unfinished at its start (0) and end (1)
   float* partial;                   // workspace: [parts][2][D / 4][256 rows][4], then [256][2] (m, l)
   float scale_log2;
@@ -297,7 +299,7 @@ Q3T_DEV Segment find_tile(const PrefillArgs& a, const int32_t* before, int index
     int n = 0, first = 0, tiles = 0;
     int64_t start = 0;
     if (s >= 0) {
-      start = a.start_positions[s];
+      start = clamped_start(a.start_positions[s]);
       n = rows_of(a, s, first);
     }
     tiles = (n + span - 1) / span;
@@ -417,16 +419,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   int32_t* prefix = reinterpret_cast<int32_t*>(smem + M::kPlan);
   int32_t* before = nullptr;
   int pairs = 0;
-  if (a.parts > 0 || (a.sequences > 32 && a.sequences <= kPlanTiles)) {
+  if (a.parts > 0 || (a.sequences > 32 && a.sequences <= kPlanTiles && a.pairs <= kPlanPairs)) {
     before = a.parts > 0 ? prefix + kPlanTiles + 1 : prefix;
     const int span = 2 * a.positions;
     for (int s0 = 0; s0 < a.sequences; s0 += kThreads) {
       const int s = a.sequences - 1 - s0 - int(threadIdx.x);
       int first, n = s >= 0 ? rows_of(a, s, first) : 0, all;
-      n = (n + span - 1) / span;
+      // offsets that run backwards may make sequences overlap: no more pairs are listed than rows in order can have
+      n = min((n + span - 1) / span, a.pairs);
       const int sum = block_sum(n, bars->sums, warp, lane, all);
-      if (s >= 0) before[a.sequences - 1 - s] = pairs + sum - n;
-      pairs += all;
+      if (s >= 0) before[a.sequences - 1 - s] = min(pairs + sum - n, a.pairs);
+      pairs = min(pairs + all, a.pairs);
     }
     __syncthreads();
     int work = 0;
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int i = row_of(before, a.sequences, e, 1), s = a.sequences - 1 - i;
         int first;
         const int n = rows_of(a, s, first), tile = (n + span - 1) / span - 1 - (e - before[i]);
-        cost = kFixed + key_tiles_of(a, a.start_positions[s] + min(n, (tile + 1) * span));
+        cost = kFixed + key_tiles_of(a, clamped_start(a.start_positions[s]) + min(n, (tile + 1) * span));
       }
       const int sum = block_sum(cost, bars->sums, warp, lane, all);
       if (e < pairs) prefix[e] = work + sum - cost;
@@ -906,7 +909,7 @@ int launch_prefill(const q3t_paged_prefill& p, const PrefillArgs& a, int64_t blo
 // How a call runs, from sizes that the host knows.
 struct PrefillPlan {
   int heads, passes, positions;
-  int64_t items;  // at most: every sequence may end inside a pair of tiles
+  int64_t pairs, items;  // at most: every sequence may end inside a pair of tiles
   int parts;      // ranges; 0: one item per CTA
   size_t bytes;
 };
@@ -916,14 +919,14 @@ PrefillPlan prefill_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64
   p.heads = int(group < 64 ? group : 64);
   p.passes = int((group + p.heads - 1) / p.heads);
   p.positions = kTileRows / p.heads;
-  const int64_t pairs = rows / (2 * p.positions) + sequences;
-  p.items = pairs * kv_heads * p.passes;
+  p.pairs = rows / (2 * p.positions) + sequences;
+  p.items = p.pairs * kv_heads * p.passes;
   // Ranges pay where items are few and may be long: 4 chunks of 100..700 rows behind 2000..8000 keys 148 us in turn, 117 in
   // ranges; 512 rows behind 16000 keys 221 and 77; 1 row behind 2000 keys 30 and 24. With many items they only add the
   // plan and the join (one prompt of 4096 rows and 32 heads: 128 and 137; one of 2048 and 16 heads: 36 and 44).
   const int64_t tiles = (capacity + kTileKeys - 1) / kTileKeys, sms = sm_count();
   const bool few = (tiles >= 32 && p.items <= 3 * sms) || (tiles >= 16 && p.items <= sms / 4);
-  p.parts = few && pairs <= kPlanTiles && sequences <= kPlanSequences && pairs * (tiles + kFixed) < (int64_t(1) << 31) ? int(sms) : 0;
+  p.parts = few && p.pairs <= kPlanTiles && sequences <= kPlanSequences && p.pairs * (tiles + kFixed) < (int64_t(1) << 31) ? int(sms) : 0;
   p.bytes = p.parts == 0 ? 0 : size_t(p.parts) * 2 * (sizeof(Segment) + size_t(256) * (head_dim + 2) * 4);
   return p;
 }
@@ -969,6 +972,7 @@ int launch_prefill_tiles(const q3t_paged_prefill& p, unsigned* status, void* str
   a.status = status;
   a.out_32 = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
   a.parts = plan.parts;
+  a.pairs = int(plan.pairs);
   a.shared_segments = static_cast<Segment*>(p.workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + size_t(plan.parts) * 2 * sizeof(Segment));
   const int64_t blocks = plan.parts > 0 ? plan.parts : plan.items;

@@ -542,7 +542,7 @@ def _paged_cache(what: str, device: int, key_pages, value_pages, page_table):
             or page_table.get_device() != device):
         raise ValueError(f"{what}: expected CUDA tensors on one device")
     shape, stride = key_pages.shape, key_pages.stride()
-    if (key_pages.dtype is not BF16 or value_pages.dtype is not BF16 or len(shape) != 4 or value_pages.shape != shape
+    if (key_pages.dtype is not BF16 or value_pages.dtype is not BF16 or len(shape) != 4 or 0 in shape or value_pages.shape != shape
             or value_pages.stride() != stride):
         raise ValueError(f"{what}: expected BF16 key and value pages [pages, Hkv, page_size, D], laid out alike")
     pages, heads, size, dim = shape

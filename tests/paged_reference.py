@@ -58,7 +58,7 @@ def attend(query, keys, values, scale):
 
     bound: the weights' rounding to bf16 and the output's, 2^-8 each; a score's error is at most
     (dim + 16) steps of 2^-23 (sums that may truncate, the scale, the base-2 exponential's argument) of
-    scale * sum |q k| and of the largest score, and moves every weight by that much relative, numerator and
+    |scale| * sum |q k| and of the largest score, and moves every weight by that much relative, numerator and
     denominator both; sums of n weights and products in 32 bits add n * 2^-23 at most (twice)."""
     q_heads, dim = query.shape
     group, n = q_heads // keys.shape[0], keys.shape[1]
@@ -68,7 +68,7 @@ def attend(query, keys, values, scale):
     scores = scale * q @ keys.mT
     weights = torch.softmax(scores, -1)
     out, spread = weights @ values, weights @ values.abs()
-    size = (scale * q.abs() @ keys.abs().mT).amax(-1, keepdim=True) + scores.abs().amax(-1, keepdim=True)
+    size = (abs(scale) * q.abs() @ keys.abs().mT).amax(-1, keepdim=True) + scores.abs().amax(-1, keepdim=True)
     slack = 2 * (dim + 16) * 2.0 ** -23 * size + 2 * n * 2.0 ** -23
     # the two roundings compound: (1 + 2^-8)^2 - 1
     return out.reshape(q_heads, dim), (HALF_STEP * (1 + HALF_STEP) * (spread + out.abs())

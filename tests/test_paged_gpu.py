@@ -613,6 +613,46 @@ def test_prompts_with_odd_offsets_are_flagged(ops, cuda):
                 assert near.all() if owned else (got == 5).all(), f"{offsets} row {r}"
 
 
+@pytest.mark.parametrize("count", [400, 1200, 2500])
+def test_prompts_that_overlap_are_flagged(ops, cuda, count):
+    """Offsets 0, R, 0, R, ...: every other sequence runs backwards, the rest share all rows (and, here, their pages, so
+    that a row's result is the same whose ever it is). More tiles than rows in order can have are not looked at."""
+    rows = 8192
+    case = Case([rows], 1, 64, 64)
+    query = rows_of((rows, 1, 64), 1, False)
+    keys, values, table = case.to(cuda)
+    out = torch.full_like(query, 5.0, device=cuda)
+    ops.paged_prefill_attention(query.to(cuda), keys, values, table.repeat(count, 1),
+                                torch.tensor([0, rows] * (count // 2) + [0], device=cuda),
+                                torch.zeros(count, dtype=torch.int64, device=cuda), out=out)
+    assert ops.read_status(cuda) == 8
+    for r in [*range(0, rows, 409), rows - 1]:
+        want, bound = attend(query[r], *case.sequence(0, r + 1), 0.125)
+        assert_within(out[r], want, bound, f"row {r}")
+
+
+@pytest.mark.parametrize("scale", [0.125, -0.125])
+@pytest.mark.parametrize("columns", [3, 3000])
+def test_prompts_that_start_far_away(ops, cuda, columns, scale):
+    """Starts at the ends of 64 bits: past the table (flagged), or left padding only (zeros)."""
+    case = Case([40, 40, 40], 2, 64, 16)
+    query = rows_of((120, 4, 64), 1, False)
+    keys, values, table = case.to(cuda)
+    wide = torch.full((3, columns), -1, dtype=torch.int32, device=cuda)
+    wide[:, :3] = table
+    offsets = torch.tensor([0, 40, 80, 120], device=cuda)
+    for far, status in ((2 ** 63 - 1, 8), (2 ** 63 - 20, 8), (-2 ** 63, 0), (-2 ** 63 + 20, 0)):
+        out = torch.full_like(query, 5.0, device=cuda)
+        ops.paged_prefill_attention(query.to(cuda), keys, values, wide, offsets, torch.tensor([0, far, 0], device=cuda),
+                                    out=out, scale=scale)
+        assert ops.read_status(cuda) == status
+        if status == 0:
+            assert (out[40:80] == 0).all()
+        for r in [*range(40), *range(80, 120)]:
+            want, bound = attend(query[r], *case.sequence(r // 40, r % 40 + 1), scale)
+            assert_within(out[r], want, bound, f"row {r}")
+
+
 def test_empty_batches_and_given_outputs(ops, cuda):
     case = Case([20], 2, 64, 16)
     keys, values, table = case.to(cuda)

@@ -40,6 +40,12 @@ int main() {
   CHECK(look(0, int64_t(1) << 62) == -1 && look(0, -(int64_t(1) << 62)) == -1);
   CHECK(steps_of(-1) == 0 && steps_of(0) == 1 && steps_of(15) == 1 && steps_of(16) == 2);
 
+  // starts of packed sequences: as given while they can be, and safe to count on from
+  for (int64_t s : {int64_t(0), int64_t(-5), int64_t(1) << 35, -(int64_t(1) << 35)}) CHECK(clamped_start(s) == s);
+  const int64_t last = 9223372036854775807;
+  CHECK(clamped_start(last) + 2147483647 > (int64_t(1) << 34) && clamped_start(last) > (int64_t(1) << 34));
+  CHECK(clamped_start(-last - 1) + 2147483647 < 0);
+
   // even splits: the ranges tile [0, total), differ by one at most, and split_owner inverts them
   for (int64_t total : {1, 2, 7, 8, 9, 147, 148, 149, 1000, 4097})
     for (int64_t parts : {1, 2, 8, 148, 296, 1184}) {
@@ -177,6 +183,7 @@ def test_valid_arguments_reach_the_launch(entry, no_launch):
 
 SHARED = [dict(keys=pool(dtype=torch.float16)), dict(values=pool(heads=1)), dict(values=pool()[:, :, ::2]),
           dict(keys=pool(size=32)[:, :, ::2]), dict(keys=pool()[0]), dict(keys=pool(pages=12)[::2]),
+          dict(keys=pool(heads=0), values=pool(heads=0)), dict(keys=pool(pages=0), values=pool(pages=0)),
           dict(page_table=table(dtype=torch.int64)), dict(page_table=table(columns=4)[:, ::2]),
           dict(page_table=table(rows=2)), dict(page_table=table()[0])]
 BAD = [(decode, c) for c in SHARED + [
