@@ -403,7 +403,7 @@ typedef struct {
  * and writes its key and value at cache_positions[r]; cos/sin tables [table_len, head_dim] bf16 are
  * indexed by rotary_positions[r] (out of range: clamped, bad-index bit). A row with a negative
  * sequence is graph padding: it writes nothing and raises nothing. No two rows may name the same
- * position of a page. query_out: [rows, q_heads, head_dim]. */
+ * position of a page. query_out: [rows, q_heads, head_dim]; neither it nor the pools overlap qkv. */
 typedef struct {
   q3t_paged_cache cache;
   const void* qkv;

@@ -8,13 +8,15 @@
 //
 // The kernel is bound by its bytes: every element is read and written once. D/16 lanes own a head; a lane
 // holds 8 dims of the first half and the 8 dims that rotate with them in the second, so RoPE needs no
-// exchange between lanes and the norm only the D/16-lane sum. A lane takes HEADS heads of a row, whose loads
-// are all on their way before the first is used, and reads the row's positions, cos and sin once for them.
+// exchange between lanes and the norm only the D/16-lane sum. A lane takes HEADS heads of one kind of a row, whose
+// loads are all on their way before the first is used, and reads the row's positions, cos and sin once for them.
 //
-// 3500 rows of 16 + 2 * 8 heads of 128 dims: 17.2 us for 65.8 MB, 3.8 TB/s; 16000 rows 4.8 TB/s; 1 to 64 rows 2.5 us. The
-// same kernel that only copies takes 11 us for the 3500: what is between is the chain of positions, cos/sin and the head's
-// sum in each thread, with as many threads as the registers allow. Fewer registers (a launch bound), two or eight heads to
-// a lane, packed fp32 arithmetic, and rows brought into shared memory by a copying warp were all slower.
+// 3500 rows of 16 + 2 * 8 heads of 128 dims: 13.1 us for 65.8 MB, 5.0 TB/s; 16000 rows 5.7 TB/s; 1 to 64 rows 2.3 us. The
+// same kernel that only copies takes 10.0 us for the 3500. With the weight, cos and sin unpacked and multiplied for every
+// head the kernel was bound by its instructions (276 for a warp's four heads, 60 % of the issue slots at 17 warps per
+// SM): 17.4 us; packed arithmetic on factors that four heads share 16.2, the dependent loads first 15.2, the rows kept
+// out of L1 13.1. Two or eight heads to a lane, a loop that fetches the next heads meanwhile (two of them in registers
+// leave fewer warps), and rows brought into shared memory by a copying warp were all slower.
 #include "common.cuh"
 #include "host.cuh"
 #include "paged.cuh"
@@ -40,92 +42,128 @@ struct WriteArgs {
 
 constexpr int kThreads = 128;
 
+Q3T_DEV float2 unpack2(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+Q3T_DEV uint32_t pack2(float2 v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+struct Words {
+  uint32_t w[4];
+};
+Q3T_DEV Words load8(const __nv_bfloat16* p) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  return {{v.x, v.y, v.z, v.w}};
+}
+// The same for what is read once: it leaves L1 to the weights, cos and sin (3500 rows 15.2 -> 13.0 us).
+Q3T_DEV Words load8_once(const __nv_bfloat16* p) {
+  Words v;
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3])
+               : "l"(p)
+               : "memory");
+  return v;
+}
+Q3T_DEV void store8(__nv_bfloat16* p, const Words& v) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+}
+
 template <int D, int HEADS>
-__global__ void __launch_bounds__(kThreads) paged_write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(kThreads, HEADS == 1 ? 1 : 5) paged_write_kernel(const WriteArgs a) {
   constexpr int L = D / 16;  // lanes of a head
   grid_dependency_wait();
-  const int heads = a.q_heads + 2 * a.kv_heads, chunks = (heads + HEADS - 1) / HEADS;
+  const int q_chunks = (a.q_heads + HEADS - 1) / HEADS, kv_chunks = (a.kv_heads + HEADS - 1) / HEADS;
+  const int chunks = q_chunks + 2 * kv_chunks;
   const unsigned unit = blockIdx.x * (kThreads / L) + threadIdx.x / L;
   const unsigned r = unit / unsigned(chunks);
   if (r >= a.rows) return;  // whole groups of L lanes leave; the sums below name the lanes of a group
-  const int head0 = int(unit - r * chunks) * HEADS, d0 = int(threadIdx.x % L) * 8;
+  int chunk = int(unit - r * chunks);
+  const int kind = chunk < q_chunks ? 0 : chunk < q_chunks + kv_chunks ? 1 : 2;  // queries, keys, values
+  if (kind > 0) chunk -= q_chunks + (kind - 1) * kv_chunks;
+  const int head0 = chunk * HEADS, heads = min(HEADS, (kind > 0 ? a.kv_heads : a.q_heads) - head0);
+  const int d0 = int(threadIdx.x % L) * 8;
   const unsigned group = (L == 8 ? 0xffu : 0xfu) << (threadIdx.x & 31 & ~(L - 1));
 
-  uint4 x[HEADS][2];
-  const __nv_bfloat16* src = a.qkv + r * a.qkv_stride + int64_t(head0) * D + d0;
-#pragma unroll
-  for (int i = 0; i < HEADS; ++i) {
-    x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (head0 + i < heads) {
-      x[i][0] = *reinterpret_cast<const uint4*>(src + i * D);
-      x[i][1] = *reinterpret_cast<const uint4*>(src + i * D + D / 2);
-    }
-  }
+  // the loads that others depend on first, then all the others
   const int64_t sequence = a.sequences != nullptr ? a.sequences[r] : r;
   const int64_t position = a.cache_positions[r];
   int64_t rp = a.rotary_positions[r];
-  const bool rp_ok = rp >= 0 && rp < a.table_len;
-  if (!rp_ok) rp = rp < 0 ? 0 : a.table_len - 1;
-  float c0[8], c1[8], s0[8], s1[8];
-  unpack8(*reinterpret_cast<const uint4*>(a.cos + rp * D + d0), c0);
-  unpack8(*reinterpret_cast<const uint4*>(a.cos + rp * D + D / 2 + d0), c1);
-  unpack8(*reinterpret_cast<const uint4*>(a.sin + rp * D + d0), s0);
-  unpack8(*reinterpret_cast<const uint4*>(a.sin + rp * D + D / 2 + d0), s1);
-  if (sequence < 0) return;  // padding
-  if (!rp_ok && head0 == 0 && d0 == 0) raise_status(a.status, kStatusBadIndex);
-  int64_t at = -1;  // element offset of the row's position in a pool, head 0
-  if (head0 + HEADS > a.q_heads) {
-    int row;
-    const int64_t page = a.pages.lookup(sequence, position, row);
-    if (page >= 0) at = page * a.page_stride + int64_t(row) * D + d0;
-    else if (d0 == 0) raise_status(a.status, kStatusBadIndex);
-  }
+  Words x[HEADS][2];
+  const int in_row = head0 + (kind > 0 ? a.q_heads + (kind - 1) * a.kv_heads : 0);
+  const __nv_bfloat16* src = a.qkv + r * a.qkv_stride + int64_t(in_row) * D + d0;
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
-    const int head = head0 + i;
-    if (head >= heads) break;
-    __nv_bfloat16* dst = a.query_out + (int64_t(r) * a.q_heads + head) * D + d0;
-    if (head >= a.q_heads) {
-      const bool key = head < a.q_heads + a.kv_heads;
-      const int h = head - a.q_heads - (key ? 0 : a.kv_heads);
-      if (at < 0) continue;
-      dst = (key ? a.key_pages : a.value_pages) + at + int64_t(h) * a.pages.page_size * D;
-    }
-    if (head < a.q_heads + a.kv_heads) {
-      float y0[8], y1[8], o0[8], o1[8];
-      unpack8(x[i][0], y0);
-      unpack8(x[i][1], y1);
-      if (a.q_norm != nullptr) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += y0[e] * y0[e] + y1[e] * y1[e];
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
-        const float inv = rsqrtf(ss * (1.f / float(D)) + a.eps);
-        const __nv_bfloat16* w = head < a.q_heads ? a.q_norm : a.k_norm;
-        float w0[8], w1[8];
-        unpack8(*reinterpret_cast<const uint4*>(w + d0), w0);
-        unpack8(*reinterpret_cast<const uint4*>(w + D / 2 + d0), w1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y0[e] *= inv * w0[e], y1[e] *= inv * w1[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        o0[e] = y0[e] * c0[e] - y1[e] * s0[e];
-        o1[e] = y1[e] * c1[e] + y0[e] * s1[e];
-      }
-      x[i][0] = pack8(o0);
-      x[i][1] = pack8(o1);
-    }
-    *reinterpret_cast<uint4*>(dst) = x[i][0];
-    *reinterpret_cast<uint4*>(dst + D / 2) = x[i][1];
+    x[i][0] = x[i][1] = {};
+    if (i < heads) x[i][0] = load8_once(src + i * D), x[i][1] = load8_once(src + i * D + D / 2);
   }
+  const bool rp_ok = rp >= 0 && rp < a.table_len;
+  if (!rp_ok) rp = rp < 0 ? 0 : a.table_len - 1;
+  Words c0 = {}, c1 = {}, s0 = {}, s1 = {};
+  if (kind < 2) {
+    c0 = load8(a.cos + rp * D + d0), c1 = load8(a.cos + rp * D + D / 2 + d0);
+    s0 = load8(a.sin + rp * D + d0), s1 = load8(a.sin + rp * D + D / 2 + d0);
+  }
+  __nv_bfloat16* dst = a.query_out + (int64_t(r) * a.q_heads + head0) * D + d0;
+  int64_t step = D;  // from head to head
+  if (kind > 0) {
+    int row;
+    const int64_t page = a.pages.lookup(sequence, position, row);
+    step *= a.pages.page_size;
+    dst = page < 0 ? nullptr : (kind == 1 ? a.key_pages : a.value_pages) + page * a.page_stride + head0 * step + row * D + d0;
+  }
+  if (sequence < 0) return;  // padding
+  if (d0 == 0 && (dst == nullptr || (!rp_ok && kind == 0 && head0 == 0))) raise_status(a.status, kStatusBadIndex);
+  if (dst == nullptr) return;
+
+  if (kind < 2) {
+    // o0 = inv (x0 a + x1 b), o1 = inv (x1 c + x0 d): the weight goes into cos and sin once for the lane's heads, and inv
+    // comes last, behind products that do not wait for the sum
+    float2 fa[4], fb[4], fc[4], fd[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      fa[e] = unpack2(c0.w[e]), fb[e] = unpack2(s0.w[e] ^ 0x80008000u);  // -sin
+      fc[e] = unpack2(c1.w[e]), fd[e] = unpack2(s1.w[e]);
+    }
+    if (a.q_norm != nullptr) {
+      const __nv_bfloat16* w = kind == 0 ? a.q_norm : a.k_norm;
+      const Words w0 = load8(w + d0), w1 = load8(w + D / 2 + d0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 u = unpack2(w0.w[e]), v = unpack2(w1.w[e]);
+        fa[e] = mul2(fa[e], u), fd[e] = mul2(fd[e], u);
+        fb[e] = mul2(fb[e], v), fc[e] = mul2(fc[e], v);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+      float2 x0[4], x1[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x0[e] = unpack2(x[i][0].w[e]), x1[e] = unpack2(x[i][1].w[e]);
+      float inv = 1.f;
+      if (a.q_norm != nullptr) {
+        float2 squares = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) squares = fma2(x1[e], x1[e], fma2(x0[e], x0[e], squares));
+        float sum = squares.x + squares.y;
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(group, sum, o);
+        inv = rsqrtf(sum * (1.f / float(D)) + a.eps);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[i][0].w[e] = pack2(mul2(fma2(x0[e], fa[e], mul2(x1[e], fb[e])), {inv, inv}));
+        x[i][1].w[e] = pack2(mul2(fma2(x1[e], fc[e], mul2(x0[e], fd[e])), {inv, inv}));
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i)
+    if (i < heads) store8(dst + i * step, x[i][0]), store8(dst + i * step + D / 2, x[i][1]);
 }
 
 template <int D, int HEADS>
 int launch_write(const WriteArgs& a, void* stream, const char* name) {
   constexpr int kUnits = kThreads / (D / 16);
-  const int64_t units = a.rows * ((a.q_heads + 2 * a.kv_heads + HEADS - 1) / HEADS);
+  const int64_t units = a.rows * ((a.q_heads + HEADS - 1) / HEADS + 2 * ((a.kv_heads + HEADS - 1) / HEADS));
   return launch(paged_write_kernel<D, HEADS>, dim3(unsigned((units + kUnits - 1) / kUnits)), dim3(kThreads), 0, stream, true,
                 name, a);
 }
@@ -173,9 +211,10 @@ extern "C" int q3t_paged_qk_norm_rope_kv(const q3t_paged_write* call, unsigned* 
   a.kv_heads = int(c.kv_heads);
   a.rows = p.rows;
   a.status = status;
-  // few rows: a lane per head for the shortest chain (1..64 rows of 32 heads 2.5 us against 3.7 with four); many: four
-  // heads to a lane (3500 rows 17.2 us against 19.2)
-  const bool few = p.rows * heads <= 32768;
+  // few rows: a lane per head for the shortest chain (64 rows of 32 heads 2.4 us against 3.2 with four, 512 rows 3.4
+  // against 3.7); many: four heads to a lane share what a row needs once (1000 rows 5.1 us against 5.4, 3500 13.1
+  // against 16.5)
+  const bool few = p.rows * heads <= 24576;
   if (c.head_dim == 128) return few ? launch_write<128, 1>(a, stream, name) : launch_write<128, 4>(a, stream, name);
   return few ? launch_write<64, 1>(a, stream, name) : launch_write<64, 4>(a, stream, name);
 }
