@@ -270,12 +270,57 @@ Q3T_DEV void rest(const Run<D>& run, float* part, int heads, int g, int t) {
 // One CTA per (row, key/value head, pass), or a cluster of `ranks`: the warps share the row's steps in contiguous runs,
 // merge through shared memory, and a cluster's CTAs through distributed shared memory. 256 rows of 1..4096 keys, 16 query
 // and 8 KV heads of 128 dims: 313 us for 2.17 GB, 6.9 TB/s (a plain read of memory reaches 7.1).
-// PROMPT: row r is a packed prompt row, whose sequence and position follow from row_offsets and start_positions; this is
-// the form of the prompt attention for what its tiled kernel does not take.
+// PROMPT: row r is a packed prompt row, whose sequence and position follow from row_offsets and start_positions: the form
+// of the prompt attention for few rows and for what its tiled kernel does not take (prompt_by_rows).
 struct PromptRows {
   const int64_t *row_offsets, *start_positions;
   int sequences;
 };
+constexpr int kLookRounds = 4;  // of 32 sequences, looked at at once
+
+// Position of packed row `row` in its sequence (below -1 as -1), for a whole warp; false: no sequence owns it. Offsets
+// that make no sense are flagged by the first CTA and own nothing. Up to 128 sequences take one round of loads where a
+// search takes one for each halving.
+Q3T_DEV bool locate(const PromptRows& pr, int rows, int row, bool first, unsigned* status, int64_t& sequence, int64_t& position) {
+  const int lane = threadIdx.x & 31;
+  sequence = -1;
+  if (pr.sequences <= 32 * kLookRounds) {
+    int64_t lo[kLookRounds], hi[kLookRounds], start[kLookRounds];
+#pragma unroll
+    for (int i = 0; i < kLookRounds; ++i) {
+      const int s = 32 * i + lane;
+      lo[i] = hi[i] = start[i] = 0;
+      if (s < pr.sequences) lo[i] = pr.row_offsets[s], hi[i] = pr.row_offsets[s + 1], start[i] = pr.start_positions[s];
+    }
+#pragma unroll
+    for (int i = 0; i < kLookRounds; ++i) {
+      const bool sound = lo[i] >= 0 && lo[i] <= hi[i] && hi[i] <= rows;
+      if (first && !sound) raise_status(status, kStatusBadIndex);
+      const unsigned hit = __ballot_sync(0xffffffffu, sound && lo[i] <= row && row < hi[i]);
+      if (hit == 0 || sequence >= 0) continue;
+      sequence = 32 * i + __ffs(hit) - 1;
+      position = __shfl_sync(0xffffffffu, clamped_start(start[i]) + (row - lo[i]), __ffs(hit) - 1);
+    }
+  } else {
+    int lo = 0, hi = pr.sequences;  // the last sequence that starts at or before the row
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pr.row_offsets[mid] <= row) lo = mid;
+      else hi = mid;
+    }
+    const int64_t begin = pr.row_offsets[lo], end = pr.row_offsets[lo + 1];
+    if (begin >= 0 && begin <= row && row < end && end <= rows) {
+      sequence = lo;
+      position = clamped_start(pr.start_positions[lo]) + (row - begin);
+    }
+    for (int s = threadIdx.x; first && s < pr.sequences; s += blockDim.x)
+      if (pr.row_offsets[s] < 0 || pr.row_offsets[s] > pr.row_offsets[s + 1] || pr.row_offsets[s + 1] > rows)
+        raise_status(status, kStatusBadIndex);
+  }
+  if (sequence < 0) return false;
+  if (position < 0) position = -1;
+  return true;
+}
 
 template <int D, int W, int ST, bool PROMPT>
 __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct(const DecodeArgs a, const PromptRows pr) {
@@ -289,16 +334,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
   const int head = unit / a.passes, pass = unit % a.passes;
   int64_t sequence = row, position;
   if constexpr (PROMPT) {
-    int lo = 0, hi = pr.sequences;  // the last sequence that starts at or before the row
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pr.row_offsets[mid] <= row) lo = mid;
-      else hi = mid;
-    }
-    if (row < pr.row_offsets[lo] || row >= pr.row_offsets[lo + 1]) return;  // a row of no sequence
-    sequence = lo;
-    position = clamped_start(pr.start_positions[lo]) + (row - pr.row_offsets[lo]);
-    if (position < 0) position = -1;
+    if (!locate(pr, a.rows, row, blockIdx.x == 0, a.status, sequence, position)) return;  // the same for a cluster's CTAs
   } else {
     position = a.positions[row];
   }
@@ -802,6 +838,17 @@ DecodePlan decode_plan(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t 
   return p;
 }
 
+// Whether prompt rows go row by row, as in a decode call, instead of in tiles. A tile takes as long for one row as for
+// 128, but a row's keys are read for that row alone. With 16 query and 8 KV heads of 128 dims, tiles and rows: one prompt
+// of 13 rows 7.2 us and 3.9; 48 rows 7.4 and 4.4, 64 rows even; 4 rows behind 4000 keys 25.7 and 9.5; 16 rows behind 500
+// 13.7 and 6.6, behind 4000 25.9 and 21.4, behind 8000 32.6 and 38.9; 48 rows behind 1000 20.1 and 16.1, 24 behind 2000
+// 22.8 and 20.6. The host knows the table's columns only, not the rows' keys.
+bool prompt_by_rows(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t capacity) {
+  const DecodePlan p = decode_plan(rows, q_heads, kv_heads, 1);
+  const int64_t items = rows * kv_heads * ((q_heads / kv_heads + kHeads - 1) / kHeads);
+  return items <= 3 * sm_count() && capacity <= (p.wide ? 6144 * p.ranks : 2048);
+}
+
 template <int D, int W, int ST>
 int launch_split(const DecodeArgs& a, void* workspace, void* stream, const char* name) {
   static PerDevice once;
@@ -887,7 +934,9 @@ extern "C" int q3t_paged_decode_attention(const q3t_paged_decode* call, unsigned
 extern "C" size_t q3t_paged_prefill_attention_workspace_bytes(int64_t rows, int64_t sequences, int64_t q_heads,
                                                               int64_t kv_heads, int64_t head_dim, int64_t context) {
   if (rows < 1 || sequences < 1 || q_heads < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
-  return prefill_tiles_workspace(rows, sequences, q_heads, kv_heads, head_dim, context);
+  return prompt_by_rows(rows, q_heads, kv_heads, context)
+             ? 0
+             : prefill_tiles_workspace(rows, sequences, q_heads, kv_heads, head_dim, context);
 }
 
 extern "C" int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsigned* status, void* stream) {
@@ -901,8 +950,14 @@ extern "C" int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsign
     return fail(Q3T_EINVAL, "%s: invalid geometry", name);
   const DeviceGuard guard(p.cache.device);
   if (!guard.ok()) return fail(Q3T_ECUDA, "%s: no such device", name);
-  if (prefill_tiles_supported(p)) return launch_prefill_tiles(p, status, stream, name);
+  const bool by_rows = prompt_by_rows(p.rows, p.q_heads, p.cache.kv_heads, a.context);
+  if (!by_rows && prefill_tiles_supported(p)) return launch_prefill_tiles(p, status, stream, name);
   const PromptRows pr = {p.row_offsets, p.start_positions, int(p.sequences)};
-  return p.cache.head_dim == 128 ? launch_direct<128, 8, 2, true>(a, pr, 1, stream, name)
-                                 : launch_direct<64, 8, 4, true>(a, pr, 1, stream, name);
+  const DecodePlan how = decode_plan(p.rows, p.q_heads, p.cache.kv_heads, 1);
+  const bool d128 = p.cache.head_dim == 128;
+  if (how.wide || !by_rows)
+    return d128 ? launch_direct<128, 8, 2, true>(a, pr, how.ranks, stream, name)
+                : launch_direct<64, 8, 4, true>(a, pr, how.ranks, stream, name);
+  return d128 ? launch_direct<128, 4, 2, true>(a, pr, 1, stream, name)
+              : launch_direct<64, 4, 4, true>(a, pr, 1, stream, name);
 }

@@ -903,7 +903,7 @@ PrefillPlan prefill_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64
   p.pairs = rows / (2 * p.positions) + sequences;
   p.items = p.pairs * kv_heads * p.passes;
   // Ranges pay where items are few and may be long: 4 chunks of 100..700 rows behind 2000..8000 keys 148 us in turn, 117 in
-  // ranges; 512 rows behind 16000 keys 221 and 77; 1 row behind 2000 keys 30 and 24. With many items they only add the
+  // ranges; 512 rows behind 16000 keys 221 and 77. With many items they only add the
   // plan and the join (one prompt of 4096 rows and 32 heads: 128 and 137; one of 2048 and 16 heads: 36 and 44).
   const int64_t tiles = (capacity + kTileKeys - 1) / kTileKeys, sms = sm_count();
   const bool few = (tiles >= 32 && p.items <= 3 * sms) || (tiles >= 16 && p.items <= sms / 4);

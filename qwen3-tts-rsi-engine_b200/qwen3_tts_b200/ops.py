@@ -684,7 +684,9 @@ def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offse
     Sequence s owns query rows row_offsets[s] .. row_offsets[s + 1] - 1; its i-th row has position
     start_positions[s] + i (start > 0: a chunk after a cached prefix; negative positions are left padding and
     give zeros) and sees keys 0 .. that position in the pages of page_table[s], which hold them already and finite.
-    Rows that no sequence owns are left as they are in `out`, which must not overlap query or pages. `workspace`: as for paged_decode_attention."""
+    Rows that no sequence owns are left as they are in `out`, which must not overlap query or pages. The table's columns
+    bound the context: with a view of fewer (page_table[:, :n]) few rows take the form for short contexts. `workspace`: as
+    for paged_decode_attention."""
     what = "paged_prefill_attention"
     device = query.get_device()
     cache = _paged_cache(what, device, key_pages, value_pages, page_table)

@@ -348,6 +348,87 @@ def test_prompt_sequences_of_many_lengths(ops, cuda):
     check_prompt(ops, cuda, 4, 2, 128, 16, [(13 * i) % 41 for i in range(120)], [(5 * i) % 23 for i in range(120)])
 
 
+@pytest.mark.parametrize("q,kv,d", [g for g in GEOMETRIES if g[1] < 8])
+def test_prompt_heads_in_tiles(ops, cuda, q, kv, d):
+    check_prompt(ops, cuda, q, kv, d, 32, [1, 33, 470, 5], [0, 0, 0, 40], lead=1, tail=2)
+
+
+def test_prompt_wide_groups_in_tiles(ops, cuda):
+    check_prompt(ops, cuda, 70, 1, 64, 16, [5, 140], [0, 3])
+
+
+# few rows: one CTA, or a cluster, for each row and KV head
+@pytest.mark.parametrize("counts,starts", [([1], [5000]), ([1], [0]), ([2], [700]), ([4], [4000]), ([9], [-4]), ([18], [120]),
+                                           ([3, 0, 1], [2000, 0, 100]), ([1] * 9, [513] * 9), ([0, 0, 5, 0], [0, 3, 60, 0]),
+                                           ([48], [0]), ([20, 30], [100, 9])])
+@pytest.mark.parametrize("q,kv,d,page", [(16, 8, 128, 64), (8, 8, 64, 16), (16, 1, 128, 48), (9, 1, 64, 256)])
+def test_prompt_of_few_rows(ops, cuda, counts, starts, q, kv, d, page):
+    check_prompt(ops, cuda, q, kv, d, page, counts, starts, lead=2, tail=1, strided=True)
+
+
+@pytest.mark.parametrize("count", [31, 33, 64, 127, 128, 129, 300])
+def test_prompt_of_few_rows_among_many_sequences(ops, cuda, count):
+    counts, starts = [int(i % 3 == 1) + int(i == count - 1) for i in range(count)], [(7 * i) % 90 for i in range(count)]
+    check_prompt(ops, cuda, 4, 2, 128, 16, counts, starts, lead=1, tail=2)
+
+
+@pytest.mark.parametrize("rows,ranks", [(1, 8), (3, 4), (9, 2), (18, 1)])
+@pytest.mark.parametrize("past", [0, 1])
+def test_prompt_on_either_side_of_the_limit_for_rows(ops, cuda, rows, ranks, past):
+    """16 query and 8 KV heads: by rows up to 6144 keys a CTA of the table, in tiles past them; the same results."""
+    check_prompt(ops, cuda, 16, 8, 128, 64, [rows], [1500], columns=6144 * ranks // 64 + past)
+
+
+def test_prompts_of_few_rows_with_odd_offsets_are_flagged(ops, cuda):
+    case = Case([8, 8, 8], 2, 64, 16)
+    query = rows_of((12, 4, 64), 1, False)
+    keys, values, table = case.to(cuda)
+
+    def prompt(offsets, page_table):
+        out = torch.full_like(query, 5.0, device=cuda)
+        ops.paged_prefill_attention(query.to(cuda), keys, values, page_table, torch.tensor(offsets, device=cuda),
+                                    torch.zeros(len(offsets) - 1, dtype=torch.int64, device=cuda), out=out)
+        return out, ops.read_status(cuda)
+
+    for offsets in ([0, 4, 8, 13], [-1, 4, 8, 12], [0, 6, 3, 9], [0, 2 ** 40, 8, 12]):
+        out, status = prompt(offsets, table)
+        assert status == 8
+        owners = [s for s in range(3) if 0 <= offsets[s] < offsets[s + 1] <= 12]
+        for r in range(12):
+            mine = [s for s in owners if offsets[s] <= r < offsets[s + 1]]
+            near = [(out[r].double().cpu() - want).abs() <= bound for want, bound in
+                    (attend(query[r], *case.sequence(s, r - offsets[s] + 1), 0.125) for s in mine)]
+            assert torch.stack(near).any(0).all() if mine else (out[r] == 5).all(), f"{offsets} row {r}"
+    many = [0, 4] + [8] * 149   # past the sequences that one look takes
+    assert prompt(many, table.repeat(50, 1))[1] == 0
+    for at, value in ((1, -3), (0, -1), (70, 13), (150, 13), (149, 0)):
+        out, status = prompt(many[:at] + [value] + many[at + 1:], table.repeat(50, 1))
+        assert status == 8 and (out[8:] == 5).all()
+
+
+def test_prompts_of_few_rows_repeat_captured_and_in_clusters(ops, cuda):
+    case = Case([3003, 2002], 8, 128, 64)
+    query = rows_of((5, 16, 128), 1, False).to(cuda)
+    keys, values, table = case.to(cuda)
+    offsets, starts = torch.tensor([0, 3, 5], device=cuda), torch.tensor([3000, 2000], device=cuda)
+    out = torch.empty_like(query)
+    want = ops.paged_prefill_attention(query, keys, values, table, offsets, starts, out=out).clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_prefill_attention(query, keys, values, table, offsets, starts, out=out)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    # the same keys one new token at a time
+    for r, s in enumerate((0, 0, 0, 1, 1)):
+        at = starts[s:s + 1] + (r - int(offsets[s]))
+        alone = ops.paged_decode_attention(query[r:r + 1], keys, values, table[s:s + 1], at)
+        wanted, bound = attend(query[r].cpu(), *case.sequence(s, int(at) + 1), 128 ** -0.5)
+        assert_within(alone[0], wanted, bound, f"row {r} alone")
+        assert_within(want[r], wanted, bound, f"row {r}")
+
+
 def test_prompt_scale(ops, cuda):
     check_prompt(ops, cuda, 16, 8, 128, 16, [150], [0], scale=0.5)
     check_prompt(ops, cuda, 16, 8, 128, 16, [150], [0], scale=-0.25)
