@@ -69,7 +69,8 @@ struct Segment {
   int head, head0, heads;              // KV head; first query head and query heads of the pass
   int tile0, key_tiles, all_tiles;     // key tiles of the run, and of the item
   int slot;                            // -1: the whole item; else where the run's O, m and l wait for the join
-  int64_t position;                    // of the first row
+  int position;                        // of the first row (a start past +-2^30 as that)
+  int tiles[2], keys;                  // key tiles of each query tile, and keys, counted from the run's first key on
 };
 
 template <int D>
@@ -301,7 +302,9 @@ Q3T_DEV Segment find_tile(const PrefillArgs& a, const int32_t* before, int index
     t.sequence = base - src;
     t.row = __shfl_sync(0xffffffffu, first + in_sequence, src);
     t.count = __shfl_sync(0xffffffffu, min(span, n - in_sequence), src);
-    t.position = __shfl_sync(0xffffffffu, start + in_sequence, src);
+    // no table holds 2^30 positions and no call has as many rows: 32 bits tell all that matters
+    const int64_t most = int64_t(1) << 30;
+    t.position = __shfl_sync(0xffffffffu, int(max(-most, min(most, start + in_sequence))), src);
     t.all_tiles = key_tiles_of(a, t.position + t.count);
     t.key_tiles = t.all_tiles;
     t.slot = -1;
@@ -313,6 +316,18 @@ Q3T_DEV Segment find_tile(const PrefillArgs& a, const int32_t* before, int index
     break;
   }
   return t;
+}
+
+// Completes a run: what its query tiles see of it. One warp does it for all others, off their way.
+Q3T_DEV void shape(const PrefillArgs& a, Segment& t) {
+  t.keys = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int count = max(0, min(a.positions, t.count - i * a.positions));
+    const int end = count > 0 ? keys_of(a, t.position + i * a.positions + count) - t.tile0 * kTileKeys : 0;
+    t.tiles[i] = max(0, min(t.key_tiles, (end + kTileKeys - 1) / kTileKeys));
+    t.keys = max(t.keys, min(end, t.key_tiles * kTileKeys));
+  }
 }
 
 // Inclusive sum over the CTA; `sums` holds one value per warp.
@@ -363,8 +378,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = a.kv_heads * a.passes;
   int given = 0;  // warp 3: segments handed out
-  grid_dependency_wait();
-  if (warp == 3) {
+  // set up while the launch before may still run: none of it reads what that one writes
+  if (warp == 1) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bars->q_full[i], 1);
@@ -387,13 +402,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->done, 1);
       fence_mbar_init();
     }
-  } else if (warp == 2) {
-    tmem_alloc(&bars->tmem, 512);
-    tmem_relinquish();
   } else if (warp == 0 && lane == 0) {
     prefetch_tmap(&tmq);
     prefetch_tmap(&tmk);
     prefetch_tmap(&tmv);
+  }
+  __syncthreads();
+  grid_dependency_wait();
+  if (warp == 2) {  // behind the wait: the launch before may need the columns until its end
+    tmem_alloc(&bars->tmem, 512);
+    tmem_relinquish();
   }
   // ---- the plan: the numbers behind every sequence, where it takes more than a look to find one; for ranges, the work
   // before every query tile pair, for one unit
@@ -430,7 +448,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (a.parts > 0 && threadIdx.x == 0) prefix[pairs] = work;
   }
   if (a.parts == 0 && warp == 3) {  // the CTA's first item
-    const Segment seg = find_tile(a, before, int(blockIdx.x) / units, int(blockIdx.x) % units, lane);
+    Segment seg = find_tile(a, before, int(blockIdx.x) / units, int(blockIdx.x) % units, lane);
+    shape(a, seg);
     if (lane == 0 && seg.count > 0) {
       bars->segments[0] = seg;
       mbar_arrive(&bars->segment_full[0]);
@@ -442,29 +461,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
 
-  // the next segment of work, for one warp; false: none, or a wait gave up
+  // The next segment of work, for one warp, read where it stands (the softmax loop needs every register, and a copy is
+  // on the way of the first loads) and handed back with `leave`; null: none, or a wait gave up.
   int taken = 0;
-  auto take = [&](Segment& seg, bool& ok) {
-    ok = warp_wait(&bars->segment_full[taken & 1], taken >> 1, a.status, kStatusFlagTimeout);
-    if (!ok) return false;
-    seg = bars->segments[taken & 1];
+  auto take = [&](bool& ok) -> const Segment* {
+    ok = ok && warp_wait(&bars->segment_full[taken & 1], taken >> 1, a.status, kStatusFlagTimeout);
+    const Segment* seg = &bars->segments[taken & 1];
+    return ok && seg->count > 0 ? seg : nullptr;
+  };
+  auto leave = [&] {
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->segment_free[taken & 1]);
     ++taken;
-    return seg.count > 0;
   };
-  // rows and key tiles of each of its query tiles, and its keys, numbered from its first key tile on
-  auto shape = [&](const Segment& seg, int (&count)[2], int (&tiles)[2], int& keys) {
-    keys = 0;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      count[t] = max(0, min(a.positions, seg.count - t * a.positions));
-      const int end = count[t] > 0 ? keys_of(a, seg.position + t * a.positions + count[t]) - seg.tile0 * kTileKeys : 0;
-      tiles[t] = max(0, min(seg.key_tiles, (end + kTileKeys - 1) / kTileKeys));
-      keys = max(keys, min(end, seg.key_tiles * kTileKeys));
-    }
-  };
-  int count[2], tiles[2], keys;
   bool ok = true;
 
   if (warp >= 4) {
@@ -475,17 +484,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_at = lanes + 128 * t;  // this tile's scores and weights; its output 256 columns on
     const int p = m / a.heads, h = m - p * a.heads;
     int done = 0, outs = 0;  // key tiles and outputs so far
-    for (;; ++taken) {
-      ok = warp_wait(&bars->segment_full[taken & 1], taken >> 1, a.status, kStatusFlagTimeout);
-      // read where it stands, and again after the key tiles: their loop needs every register
-      const Segment& seg = bars->segments[taken & 1];
-      if (!ok || seg.count == 0) break;
+    while (const Segment* taken_segment = take(ok)) {
+      const Segment& seg = *taken_segment;
       int key_tiles, seen0;  // of this query tile; keys that the row sees from the segment's first on
       {
-        shape(seg, count, tiles, keys);
-        key_tiles = tiles[t];
-        const int64_t position = seg.position + t * a.positions + p;
-        seen0 = int(position < -1 ? -1 : position < a.capacity ? position : a.capacity - 1) + 1 - seg.tile0 * kTileKeys;
+        key_tiles = seg.tiles[t];
+        const int position = seg.position + t * a.positions + p;
+        seen0 = max(-1, min(position, a.capacity - 1)) + 1 - seg.tile0 * kTileKeys;
       }
       float top = -INFINITY, sum = 0.f;
       for (int j = 0; j < key_tiles; ++j, ++done) {
@@ -598,19 +603,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc_fence_before();
       if (key_tiles > 0) mbar_arrive(&bars->o_free[t]);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->segment_free[taken & 1]);
+      leave();
     }
     tc_fence_before();
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLoad));
-    Segment seg;
     if (warp == 0) {
       // ---------------- loads. Lane: (piece of a key tile, 64-dim block)
       const int pieces = kTileKeys / a.piece, piece = lane / kHalves, half = lane % kHalves;
       int n = 0, loaded = 0, queries[2] = {0, 0};  // key tiles so far; loads begun; query tiles so far
-      while (ok && take(seg, ok)) {
-        shape(seg, count, tiles, keys);
+      while (const Segment* taken_segment = take(ok)) {
+        const Segment& seg = *taken_segment;
+        const int keys = seg.keys;
         const int key0 = seg.tile0 * kTileKeys;
         auto page_of = [&](int j) {  // the page of this lane's piece of tile j, and its row there
           int2 at = make_int2(int(a.pages.pages), 0);  // past the pool: a load of zeros
@@ -624,8 +628,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           return at;
         };
         int2 next = page_of(0);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (tiles[t] == 0) continue;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!ok || seg.tiles[t] == 0) continue;
           if (queries[t] > 0) ok = warp_wait(&bars->q_free[t], queries[t] - 1, a.status, kStatusMmaTimeout);
           if (!ok) break;
           ++queries[t];
@@ -657,7 +662,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (j + 1 < seg.key_tiles) next = page_of(j + 1);
         }
+        if (!ok) break;
         if (lane == 0) mbar_arrive(&bars->loaded);
+        leave();
       }
       if (!ok) {  // loads still in flight land before the CTA leaves
         for (int t = 0; t < 2; ++t)
@@ -683,12 +690,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         commit_if(&bars->s_full[t], leader);
       };
-      while (ok && take(seg, ok)) {
-        shape(seg, count, tiles, keys);
+      while (const Segment* taken_segment = take(ok)) {
+        const Segment& seg = *taken_segment;
         const int key_tiles = __shfl_sync(0xffffffffu, seg.key_tiles, 0);  // so that the compiler knows them uniform
-        tiles[0] = __shfl_sync(0xffffffffu, tiles[0], 0);
-        tiles[1] = __shfl_sync(0xffffffffu, tiles[1], 0);
-        keys = __shfl_sync(0xffffffffu, keys, 0);
+        const int tiles[2] = {__shfl_sync(0xffffffffu, seg.tiles[0], 0), __shfl_sync(0xffffffffu, seg.tiles[1], 0)};
+        const int keys = __shfl_sync(0xffffffffu, seg.keys, 0);
+        leave();
         if (key_tiles == 0) continue;
         wait(&bars->k_full[n % kStages], n / kStages, kStatusTmaTimeout);
         for (int t = 0; t < 2; ++t) {
@@ -750,7 +757,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 3) {
       // ---------------- work
-      auto give = [&](const Segment& g) {
+      Segment seg;
+      auto give = [&](Segment& g) {
+        shape(a, g);
         if (given >= 2) ok = warp_wait(&bars->segment_free[given & 1], (given >> 1) - 1, a.status, kStatusFlagTimeout);
         if (!ok) return;
         if (lane == 0) {
@@ -780,7 +789,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       } else {
-        Segment left[2] = {};  // what this range leaves to the join
+        Segment* left = a.shared_segments + blockIdx.x * 2;  // what this range leaves to the join
+        if (lane == 0) left[0].count = left[1].count = 0;
         const int64_t total = int64_t(prefix[pairs]) * units;
         const int64_t parts = split_parts(total / kLeast > 1 ? total / kLeast : 1, a.parts);
         const int64_t f1 = int64_t(blockIdx.x) < parts ? range_begin(prefix, pairs, units, blockIdx.x + 1, total, parts) : 0;
@@ -794,16 +804,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           seg.tile0 = f > item ? int(f - item) - kFixed : 0;
           seg.key_tiles = int(end - item) - kFixed - seg.tile0;
           seg.slot = f > item ? 0 : end < item + n ? 1 : -1;
-          if (seg.slot >= 0) left[seg.slot] = seg;
+          if (lane == 0 && seg.slot >= 0) left[seg.slot] = seg;
           if (seg.count > 0) give(seg);
           f = end;
         }
-        if (lane == 0) {
-          a.shared_segments[blockIdx.x * 2] = left[0];
-          a.shared_segments[blockIdx.x * 2 + 1] = left[1];
-        }
       }
-      if (ok) give(Segment{});
+      seg = {};
+      if (ok) give(seg);
     }
   }
   __syncthreads();
