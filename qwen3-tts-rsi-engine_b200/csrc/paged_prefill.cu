@@ -804,8 +804,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           seg.tile0 = f > item ? int(f - item) - kFixed : 0;
           seg.key_tiles = int(end - item) - kFixed - seg.tile0;
           seg.slot = f > item ? 0 : end < item + n ? 1 : -1;
-          if (lane == 0 && seg.slot >= 0) left[seg.slot] = seg;
           if (seg.count > 0) give(seg);
+          if (lane == 0 && seg.slot >= 0) left[seg.slot] = seg;
           f = end;
         }
       }
@@ -894,6 +894,9 @@ int launch_prefill(const q3t_paged_prefill& p, const PrefillArgs& a, int64_t blo
   return launch(paged_prefill_join<D>, dim3(unsigned(a.parts), 8), dim3(256), 0, stream, true, name, a);
 }
 
+// Bytes of the segments at the workspace's start; what follows is read and written in whole lines.
+size_t segment_bytes(int parts) { return (size_t(parts) * 2 * sizeof(Segment) + 255) / 256 * 256; }
+
 // How a call runs, from sizes that the host knows.
 struct PrefillPlan {
   int heads, passes, positions;
@@ -915,7 +918,7 @@ PrefillPlan prefill_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64
   const int64_t tiles = (capacity + kTileKeys - 1) / kTileKeys, sms = sm_count();
   const bool few = (tiles >= 32 && p.items <= 3 * sms) || (tiles >= 16 && p.items <= sms / 4);
   p.parts = few && p.pairs <= kPlanTiles && sequences <= kPlanSequences && p.pairs * (tiles + kFixed) < (int64_t(1) << 31) ? int(sms) : 0;
-  p.bytes = p.parts == 0 ? 0 : size_t(p.parts) * 2 * (sizeof(Segment) + size_t(256) * (head_dim + 2) * 4);
+  p.bytes = p.parts == 0 ? 0 : segment_bytes(p.parts) + size_t(p.parts) * 2 * 256 * (head_dim + 2) * 4;
   return p;
 }
 
@@ -962,7 +965,7 @@ int launch_prefill_tiles(const q3t_paged_prefill& p, unsigned* status, void* str
   a.parts = plan.parts;
   a.pairs = int(plan.pairs);
   a.shared_segments = static_cast<Segment*>(p.workspace);
-  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + size_t(plan.parts) * 2 * sizeof(Segment));
+  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + segment_bytes(plan.parts));
   const int64_t blocks = plan.parts > 0 ? plan.parts : plan.items;
   return c.head_dim == 128 ? launch_prefill<128>(p, a, blocks, stream, name) : launch_prefill<64>(p, a, blocks, stream, name);
 }
