@@ -15,14 +15,15 @@
 // row's maximum exceeds by at most 8 (powers of two), so O in TMEM is rescaled only when a maximum moves by more; O / l
 // does not depend on it. P's rounding to bf16 is that of a bf16 tensor product; S, m, l and O stay in fp32.
 //
-// One prompt of 8191 rows with 32 query and 8 KV heads of 128 dims: 440 us, 1250 TFLOP/s (512 us over seconds, under the
+// One prompt of 8191 rows with 32 query and 8 KV heads of 128 dims: 435 us, 1265 TFLOP/s (512 us over seconds, under the
 // power cap). A pair of 128 x 128 key tiles takes 3150 cycles of which the tensor cores work 2080: scores, the first half of
 // the weights, their product and the next scores wait for one another, and there is no TMEM for a third tile.
 //
 // Work comes in one of two ways (the host picks by sizes):
-// - items (query tile pair, KV head) in turn: a CTA whose item's loads are out takes over one that has not been launched
-//   yet, so items go to the SMs as those get free, and the next one's loads and first products overlap the last one's
-//   softmax and stores (16 prompts of 256 rows: 22.4 us against 23.9 with a CTA each);
+// - items (query tile pair, KV head) in turn: a CTA whose item's loads are nearly out takes over one that has not been
+//   launched yet, so items go to the SMs as those get free, and the next one's loads and first products overlap the last
+//   one's softmax and stores (16 prompts of 256 rows 20.1 us; before the hand-over was made leaner 22.4, against 23.9 with
+//   a CTA each);
 // - one even range of all items' key tiles per CTA, one CTA per SM. An item that a range covers only in part leaves O, m
 //   and l in the workspace, and a second, dependent launch joins the parts in the order of their keys (results repeat
 //   bit for bit). Parts are never smaller than kLeast tiles: short items move to one range whole.
@@ -41,6 +42,7 @@ constexpr int kStages = 2;  // of K, and of V
 constexpr int kThreads = 384;
 constexpr int kLeast = 4;          // key tiles of a part
 constexpr int kFixed = 2;          // what an item costs beside its key tiles, in key tiles
+constexpr int kAhead = 2;          // key tiles of an item that are still to be loaded when the next one is asked for
 constexpr int kPlanTiles = 2048;   // query tile pairs and sequences that a range plan holds
 constexpr int kPlanSequences = 1024;
 constexpr int kPlanPairs = 1 << 22;  // kThreads times as many are counted in 32 bits
@@ -615,6 +617,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (const Segment* taken_segment = take(ok)) {
         const Segment& seg = *taken_segment;
         const int keys = seg.keys;
+        const int signal = max(0, seg.key_tiles - 1 - kAhead);  // the tile at which the next item is asked for
+        if (signal == 0 && lane == 0) mbar_arrive(&bars->loaded);
         const int key0 = seg.tile0 * kTileKeys;
         auto page_of = [&](int j) {  // the page of this lane's piece of tile j, and its row there
           int2 at = make_int2(int(a.pages.pages), 0);  // past the pool: a load of zeros
@@ -643,6 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int j = 0; j < seg.key_tiles && ok; ++j, ++n) {
           const int s = n % kStages;
+          if (j > 0 && j == signal && lane == 0) mbar_arrive(&bars->loaded);
           const int2 at = next;
           const int wanted = min(pieces, (keys - j * kTileKeys + a.piece - 1) / a.piece);  // pieces that hold a key
           const uint32_t bytes = uint32_t(wanted * a.piece * 128 * kHalves);
@@ -663,7 +668,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j + 1 < seg.key_tiles) next = page_of(j + 1);
         }
         if (!ok) break;
-        if (lane == 0) mbar_arrive(&bars->loaded);
         leave();
       }
       if (!ok) {  // loads still in flight land before the CTA leaves
@@ -770,10 +774,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if (a.parts == 0) {
         // The first item was handed out above. More: take over CTAs of this grid that have not been launched yet, so the
-        // items still go to the SMs one by one, as those get free: asked for when an item's last loads are out.
+        // items still go to the SMs one by one, as those get free: asked for shortly before an item's last loads are out
+        // (16 prompts of 40..400 rows 22.5 us, 23.1 when asked for behind them), and never two ahead.
         int items = given;
         for (int i = 0; ok; ++i) {
           if (items > 0) ok = warp_wait(&bars->loaded, items - 1, a.status, kStatusFlagTimeout);
+          if (ok && given >= 2) ok = warp_wait(&bars->segment_free[given & 1], (given >> 1) - 1, a.status, kStatusFlagTimeout);
           if (!ok) break;
           if (lane == 0) {
             mbar_expect_tx(&bars->takeover, 16);
