@@ -166,10 +166,11 @@ Q3T_DEV void copy_step(uint32_t slot, const __nv_bfloat16* keys, const __nv_bflo
   for (int u = 0; u < D / 16; ++u) cp_async16(slot + at_lane.put_v[u % V] + u * 512, values + at + u * 256 + lane8);
 }
 
-// One step from its FIFO slot: 16 keys, of which the first `valid` count.
+// One step from its FIFO slot: 16 keys, of which the first `valid` count; `masked`: this lane's columns see only the first
+// sees.x and sees.y of them.
 template <int D>
 Q3T_DEV void attend_step(Run<D>& run, uint32_t slot, const Places<D>& at_lane, const uint4 (&q)[D / 32], int valid,
-                         float scale_log2, int g, int t) {
+                         bool masked, int2 sees, float scale_log2, int g, int t) {
   constexpr int C = D / 32;
   // ---- S^T = K Q^T; even and odd steps accumulate apart: two chains
   float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -189,9 +190,11 @@ Q3T_DEV void attend_step(Run<D>& run, uint32_t slot, const Places<D>& at_lane, c
   float p[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) p[e] = (s[0][e] + s[1][e]) * scale_log2;
-  if (valid < kStepKeys) {  // the item's last step
-    if (g >= valid) p[0] = p[1] = -INFINITY;
-    if (g + 8 >= valid) p[2] = p[3] = -INFINITY;
+  if (masked) {
+    if (g >= sees.x) p[0] = -INFINITY;
+    if (g >= sees.y) p[1] = -INFINITY;
+    if (g + 8 >= sees.x) p[2] = -INFINITY;
+    if (g + 8 >= sees.y) p[3] = -INFINITY;
     // rows past the last key may hold anything, NaN too, and 0 * NaN is NaN
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -270,21 +273,27 @@ Q3T_DEV void rest(const Run<D>& run, float* part, int heads, int g, int t) {
 // One CTA per (row, key/value head, pass), or a cluster of `ranks`: the warps share the row's steps in contiguous runs,
 // merge through shared memory, and a cluster's CTAs through distributed shared memory. 256 rows of 1..4096 keys, 16 query
 // and 8 KV heads of 128 dims: 313 us for 2.17 GB, 6.9 TB/s (a plain read of memory reaches 7.1).
-// PROMPT: row r is a packed prompt row, whose sequence and position follow from row_offsets and start_positions: the form
-// of the prompt attention for few rows and for what its tiled kernel does not take (prompt_by_rows).
+// PROMPT: the item's rows are up to `pack` consecutive packed rows of one sequence, whose heads fill the eight columns (4
+// rows of two heads): the form of the prompt attention for few rows and for what its tiled kernel does not take
+// (prompt_plan).
 struct PromptRows {
   const int64_t *row_offsets, *start_positions;
   int sequences;
+  int pack;    // rows of an item at most
+  int inverse; // (i * inverse) >> 8 is column i's row in its pack (i < 8): 256 / group rounded up, 0 for packs of one row
+  int packs;   // items of a (KV head, pass) at most
+  bool look;   // few enough sequences to look at all of them at once
 };
-constexpr int kLookRounds = 4;  // of 32 sequences, looked at at once
+constexpr int kLookRounds = 4;  // of 32 sequences
 
-// Position of packed row `row` in its sequence (below -1 as -1), for a whole warp; false: no sequence owns it. Offsets
+// Sequence, first row, row count and first position of number `index`, for a whole warp; false: there is none. Offsets
 // that make no sense are flagged by the first CTA and own nothing. Up to 128 sequences take one round of loads where a
 // search takes one for each halving.
-Q3T_DEV bool locate(const PromptRows& pr, int rows, int row, bool first, unsigned* status, int64_t& sequence, int64_t& position) {
+Q3T_DEV bool locate(const PromptRows& pr, int rows, int index, bool first, unsigned* status, int64_t& sequence, int& row,
+                    int& count, int64_t& position) {
   const int lane = threadIdx.x & 31;
   sequence = -1;
-  if (pr.sequences <= 32 * kLookRounds) {
+  if (pr.look) {
     int64_t lo[kLookRounds], hi[kLookRounds], start[kLookRounds];
 #pragma unroll
     for (int i = 0; i < kLookRounds; ++i) {
@@ -292,34 +301,48 @@ Q3T_DEV bool locate(const PromptRows& pr, int rows, int row, bool first, unsigne
       lo[i] = hi[i] = start[i] = 0;
       if (s < pr.sequences) lo[i] = pr.row_offsets[s], hi[i] = pr.row_offsets[s + 1], start[i] = pr.start_positions[s];
     }
+    int before = 0;
 #pragma unroll
     for (int i = 0; i < kLookRounds; ++i) {
+      if (32 * i >= pr.sequences) continue;
       const bool sound = lo[i] >= 0 && lo[i] <= hi[i] && hi[i] <= rows;
       if (first && !sound) raise_status(status, kStatusBadIndex);
-      const unsigned hit = __ballot_sync(0xffffffffu, sound && lo[i] <= row && row < hi[i]);
-      if (hit == 0 || sequence >= 0) continue;
-      sequence = 32 * i + __ffs(hit) - 1;
-      position = __shfl_sync(0xffffffffu, clamped_start(start[i]) + (row - lo[i]), __ffs(hit) - 1);
+      const int items = sound ? (int(hi[i] - lo[i]) + pr.pack - 1) / pr.pack : 0;
+      int sum = items;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += other;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + sum > index);
+      if (hit != 0 && sequence < 0) {
+        const int src = __ffs(hit) - 1, skip = (index - before - (sum - items)) * pr.pack;
+        sequence = 32 * i + src;
+        row = __shfl_sync(0xffffffffu, int(lo[i]) + skip, src);
+        count = __shfl_sync(0xffffffffu, min(pr.pack, int(hi[i] - lo[i]) - skip), src);
+        position = __shfl_sync(0xffffffffu, clamped_start(start[i]) + skip, src);
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
     }
   } else {
     int lo = 0, hi = pr.sequences;  // the last sequence that starts at or before the row
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (pr.row_offsets[mid] <= row) lo = mid;
+      if (pr.row_offsets[mid] <= index) lo = mid;
       else hi = mid;
     }
     const int64_t begin = pr.row_offsets[lo], end = pr.row_offsets[lo + 1];
-    if (begin >= 0 && begin <= row && row < end && end <= rows) {
+    if (begin >= 0 && begin <= index && index < end && end <= rows) {
       sequence = lo;
-      position = clamped_start(pr.start_positions[lo]) + (row - begin);
+      row = index;
+      count = 1;
+      position = clamped_start(pr.start_positions[lo]) + (index - begin);
     }
     for (int s = threadIdx.x; first && s < pr.sequences; s += blockDim.x)
       if (pr.row_offsets[s] < 0 || pr.row_offsets[s] > pr.row_offsets[s + 1] || pr.row_offsets[s + 1] > rows)
         raise_status(status, kStatusBadIndex);
   }
-  if (sequence < 0) return false;
-  if (position < 0) position = -1;
-  return true;
+  return sequence >= 0;
 }
 
 template <int D, int W, int ST, bool PROMPT>
@@ -330,25 +353,33 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
   grid_dependency_wait();
   const int units = a.kv_heads * a.passes, ranks = a.ranks;
   const int item = int(blockIdx.x) / ranks, rank = int(blockIdx.x) % ranks;
-  const int row = item / units, unit = item % units;
+  const int unit = item % units;
   const int head = unit / a.passes, pass = unit % a.passes;
-  int64_t sequence = row, position;
+  int row = item / units, count = 1;  // rows of the item
+  int64_t sequence = row, position;   // position: of the first row, then of the last
   if constexpr (PROMPT) {
-    if (!locate(pr, a.rows, row, blockIdx.x == 0, a.status, sequence, position)) return;  // the same for a cluster's CTAs
+    if (!locate(pr, a.rows, row, blockIdx.x == 0, a.status, sequence, row, count, position)) return;  // as do all its CTAs
   } else {
     position = a.positions[row];
   }
-  if (position < -1 || position >= a.context) {
+  const int64_t position0 = position;
+  position += count - 1;
+  if (position >= a.context || (!PROMPT && position < -1)) {
     if (unit == 0 && threadIdx.x == 0) raise_status(a.status, kStatusBadIndex);
     position = position < -1 ? -1 : a.context - 1;
   }
-  const int heads = min(kHeads, a.group - pass * kHeads);
+  const int heads = min(kHeads, a.group - pass * kHeads), columns = PROMPT ? count * heads : heads;
   const int head0 = head * a.group + pass * kHeads;
-  __nv_bfloat16* out = a.out + (int64_t(row) * a.q_heads + head0) * D;
+  // column i: row (of the pack) and head; where its output begins
+  auto row_of_column = [&](int i) { return PROMPT ? (i * pr.inverse) >> 8 : 0; };
+  auto out_of = [&](int i) {
+    const int r = row_of_column(i);
+    return a.out + (int64_t(row + r) * a.q_heads + head0 + i - r * heads) * D;
+  };
   const int64_t steps = steps_of(position);
   if (steps == 0) {  // nothing to see: zeros
-    for (int e = rank * W * 32 + threadIdx.x; e < heads * D / 8; e += ranks * W * 32)
-      reinterpret_cast<uint4*>(out)[e] = make_uint4(0u, 0u, 0u, 0u);
+    for (int e = rank * W * 32 + threadIdx.x; e < columns * D / 8; e += ranks * W * 32)
+      reinterpret_cast<uint4*>(out_of(e / (D / 8)))[e % (D / 8)] = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
   // the CTAs that share the row: no more than give every warp a step
@@ -358,18 +389,28 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
   const int64_t r1 = rank < sharing ? split_begin(rank + 1, steps, sharing) : steps;
   const int64_t first = r0 + split_begin(warp, r1 - r0, W), last = r0 + split_begin(warp + 1, r1 - r0, W);
   uint4 q[D / 32];
-  load_query<D>(q, a.query + row * a.query_stride + int64_t(head0) * D, heads, g, t);
+  const int row_g = row_of_column(g);
+  load_query<D>(q, a.query + (row + row_g) * a.query_stride + int64_t(head0 - row_g * heads) * D, columns, g, t);
+  // keys that columns 2t and 2t + 1 see of the item's last step (16 more of the one before)
+  int2 sees = {kStepKeys, kStepKeys};
+  if constexpr (PROMPT) {
+    auto of = [&](int i) {
+      const int64_t n = min(position0 + row_of_column(i), position) + 1 - (steps - 1) * kStepKeys;
+      return int(max(n, int64_t(-2 * kStepKeys)));
+    };
+    sees = make_int2(of(2 * t), of(2 * t + 1));
+  }
   Run<D> run;
   run.reset();
   const uint32_t ring = smem_u32(smem + warp * C::kRing);
   const Places<D> at_lane(lane);
 
   // element offset of step first + i, looked up 32 steps at a time, one per lane
-  const int count = int(last - first);
+  const int own = int(last - first);
   int64_t ahead = 0;
   auto look = [&](int i) {
     int64_t at = 0;
-    if (i + lane < count) {
+    if (i + lane < own) {
       const int64_t p0 = (first + i + lane) * kStepKeys;
       int row_there;
       int64_t page = a.pages.lookup(sequence, p0, row_there);
@@ -382,7 +423,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
     return at;
   };
   auto issue = [&](int i, uint32_t slot) {
-    if (i < count) {
+    if (i < own) {
       if ((i & 31) == 0) ahead = look(i);
       copy_step<D>(slot, a.keys, a.values, __shfl_sync(0xffffffffu, ahead, i & 31), at_lane, 8 * lane);
     }
@@ -391,20 +432,32 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
   for (int i = 0; i < ST; ++i) issue(i, ring + i * C::kStepBytes);
   const int tail = int(position % kStepKeys) + 1;
   uint32_t slot = ring;
-  for (int i = 0; i < count; ++i) {
+  for (int i = 0; i < own; ++i) {
     cp_async_wait<ST - 1>();
     __syncwarp();  // the other lanes' copies too
-    attend_step<D>(run, slot, at_lane, q, first + i + 1 == steps ? tail : kStepKeys, a.scale_log2, g, t);
+    const int valid = first + i + 1 == steps ? tail : kStepKeys;
+    if constexpr (PROMPT) {  // up to 8 consecutive positions: only the last two steps hold keys that some row does not see
+      const bool near = first + i + 2 >= steps;
+      const int more = first + i + 1 == steps ? 0 : kStepKeys;
+      attend_step<D>(run, slot, at_lane, q, valid, near, make_int2(sees.x + more, sees.y + more), a.scale_log2, g, t);
+    } else {
+      attend_step<D>(run, slot, at_lane, q, valid, valid < kStepKeys, make_int2(valid, valid), a.scale_log2, g, t);
+    }
     __syncwarp();  // every lane has read the slot
     issue(i + ST, slot);
     slot = slot + C::kStepBytes == ring + C::kRing ? ring : slot + C::kStepBytes;
   }
   run.finish();
   __syncwarp();
-  rest<D>(run, reinterpret_cast<float*>(smem + warp * C::kRing), heads, g, t);  // the FIFO is drained
+  rest<D>(run, reinterpret_cast<float*>(smem + warp * C::kRing), columns, g, t);  // the FIFO is drained
   __syncthreads();
+  // a row before the first key is zero
+  auto store = [&](int i, int d, float o0, float o1, float l) {
+    const bool none = PROMPT && position0 + row_of_column(i) < 0;
+    *reinterpret_cast<uint32_t*>(out_of(i) + d) = none ? 0u : pack2(o0 / l, o1 / l);
+  };
   float* mine = reinterpret_cast<float*>(smem + W * C::kRing);
-  for (int e = threadIdx.x; e < heads * D / 2; e += W * 32) {
+  for (int e = threadIdx.x; e < columns * D / 2; e += W * 32) {
     const int i = e / (D / 2), d = e % (D / 2) * 2;
     const float* p = reinterpret_cast<const float*>(smem) + i * (D + 2);
     constexpr int kNext = C::kRing / 4;
@@ -421,7 +474,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
       o1 += x[3 + d] * f;
     }
     if (sharing == 1) {
-      *reinterpret_cast<uint32_t*>(out + i * D + d) = pack2(o0 / l, o1 / l);
+      store(i, d, o0, o1, l);
     } else {
       float* to = mine + i * (D + 2);
       if (d == 0) to[0] = top, to[1] = l;
@@ -432,7 +485,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
   if (sharing == 1) return;
   // ---- the cluster's CTAs join their runs through distributed shared memory, in the order of their keys
   cluster_sync();
-  for (int e = rank * W * 32 + threadIdx.x; e < heads * D / 2; e += ranks * W * 32) {
+  for (int e = rank * W * 32 + threadIdx.x; e < columns * D / 2; e += ranks * W * 32) {
     const int i = e / (D / 2), d = e % (D / 2) * 2;
     const uint32_t at = smem_u32(mine + i * (D + 2));
     float m[kRanks], sum[kRanks];
@@ -456,7 +509,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) paged_attention_direct
       o0 += o[r].x * f;
       o1 += o[r].y * f;
     }
-    *reinterpret_cast<uint32_t*>(out + i * D + d) = pack2(o0 / l, o1 / l);
+    store(i, d, o0, o1, l);
   }
   cluster_sync();  // no CTA leaves while its shared memory is read
 }
@@ -468,7 +521,7 @@ int launch_direct(DecodeArgs& a, const PromptRows& pr, int ranks, void* stream, 
   if (const int rc = smem_limit(once, paged_attention_direct<D, W, ST, PROMPT>, C::kSmem, name)) return rc;
   a.ranks = ranks;
   return launch_cluster(paged_attention_direct<D, W, ST, PROMPT>,
-                        dim3(unsigned(int64_t(a.rows) * a.kv_heads * a.passes * ranks)), dim3(W * 32), size_t(C::kSmem),
+                        dim3(unsigned(int64_t(PROMPT ? pr.packs : a.rows) * a.kv_heads * a.passes * ranks)), dim3(W * 32), size_t(C::kSmem),
                         ranks, stream, name, a, pr);
 }
 
@@ -639,7 +692,8 @@ __global__ void __launch_bounds__(W * 32, 1) paged_decode_split(const DecodeArgs
     }
     cp_async_wait<ST - 1>();
     __syncwarp();  // the other lanes' copies too
-    attend_step<D>(run, slot, at_lane, q, f0 + i + 1 == end ? tail : kStepKeys, a.scale_log2, g, t);
+    const int valid = f0 + i + 1 == end ? tail : kStepKeys;
+    attend_step<D>(run, slot, at_lane, q, valid, valid < kStepKeys, make_int2(valid, valid), a.scale_log2, g, t);
     __syncwarp();  // every lane has read the slot
     issue(i + ST, slot);
     slot = slot + C::kStepBytes == ring + C::kRing ? ring : slot + C::kStepBytes;
@@ -830,7 +884,7 @@ struct DecodePlan {
 DecodePlan decode_plan(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t context) {
   const int64_t units = kv_heads * ((q_heads / kv_heads + kHeads - 1) / kHeads), items = rows * units;
   DecodePlan p = {false, 1, items <= sm_count()};
-  while (p.wide && p.ranks < kRanks && items * p.ranks * 2 <= sm_count()) p.ranks *= 2;
+  while (p.wide && p.ranks < kRanks && items * p.ranks * 2 <= sm_count() && context > 128 * p.ranks) p.ranks *= 2;
   const int64_t steps = steps_of(context - 1);
   // 32-bit step counts of a row and of one unit over all rows
   p.split = context > p.ranks * (p.wide ? 8192 : 4096) && rows <= kSplitRows && steps < (int64_t(1) << 26) &&
@@ -843,10 +897,25 @@ DecodePlan decode_plan(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t 
 // of 13 rows 7.2 us and 3.9; 48 rows 7.4 and 4.4, 64 rows even; 4 rows behind 4000 keys 25.7 and 9.5; 16 rows behind 500
 // 13.7 and 6.6, behind 4000 25.9 and 21.4, behind 8000 32.6 and 38.9; 48 rows behind 1000 20.1 and 16.1, 24 behind 2000
 // 22.8 and 20.6. The host knows the table's columns only, not the rows' keys.
-bool prompt_by_rows(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t capacity) {
-  const DecodePlan p = decode_plan(rows, q_heads, kv_heads, 1);
-  const int64_t items = rows * kv_heads * ((q_heads / kv_heads + kHeads - 1) / kHeads);
-  return items <= 3 * sm_count() && capacity <= (p.wide ? 6144 * p.ranks : 2048);
+struct PromptPlan {
+  bool by_rows, look;
+  int pack;
+  int64_t packs;
+  DecodePlan how;
+};
+PromptPlan prompt_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t capacity) {
+  const int64_t group = q_heads / kv_heads;
+  PromptPlan p;
+  p.look = sequences <= 32 * kLookRounds && rows <= (int64_t(1) << 20);
+  const int64_t units = kv_heads * ((group + kHeads - 1) / kHeads);
+  // the columns of several rows share a pass over the keys where that is long or the rows are many
+  const bool many = rows * units > 3 * sm_count() || capacity > 768;
+  p.pack = many && p.look && group <= kHeads ? int(kHeads / group) : 1;
+  // every sequence may end inside a pack
+  p.packs = rows / p.pack + sequences < rows ? rows / p.pack + sequences : rows;
+  p.how = decode_plan(p.packs, q_heads, kv_heads, capacity);
+  p.by_rows = p.packs * units <= 3 * sm_count() && capacity <= (p.how.wide ? 6144 * p.how.ranks : 2048);
+  return p;
 }
 
 template <int D, int W, int ST>
@@ -934,7 +1003,7 @@ extern "C" int q3t_paged_decode_attention(const q3t_paged_decode* call, unsigned
 extern "C" size_t q3t_paged_prefill_attention_workspace_bytes(int64_t rows, int64_t sequences, int64_t q_heads,
                                                               int64_t kv_heads, int64_t head_dim, int64_t context) {
   if (rows < 1 || sequences < 1 || q_heads < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
-  return prompt_by_rows(rows, q_heads, kv_heads, context)
+  return prompt_plan(rows, sequences, q_heads, kv_heads, context).by_rows
              ? 0
              : prefill_tiles_workspace(rows, sequences, q_heads, kv_heads, head_dim, context);
 }
@@ -950,12 +1019,13 @@ extern "C" int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsign
     return fail(Q3T_EINVAL, "%s: invalid geometry", name);
   const DeviceGuard guard(p.cache.device);
   if (!guard.ok()) return fail(Q3T_ECUDA, "%s: no such device", name);
-  const bool by_rows = prompt_by_rows(p.rows, p.q_heads, p.cache.kv_heads, a.context);
-  if (!by_rows && prefill_tiles_supported(p)) return launch_prefill_tiles(p, status, stream, name);
-  const PromptRows pr = {p.row_offsets, p.start_positions, int(p.sequences)};
-  const DecodePlan how = decode_plan(p.rows, p.q_heads, p.cache.kv_heads, 1);
+  const PromptPlan plan = prompt_plan(p.rows, p.sequences, p.q_heads, p.cache.kv_heads, a.context);
+  if (!plan.by_rows && prefill_tiles_supported(p)) return launch_prefill_tiles(p, status, stream, name);
+  const PromptRows pr = {p.row_offsets, p.start_positions, int(p.sequences), plan.pack,
+                         plan.pack > 1 ? int(255 / a.group + 1) : 0, int(plan.packs), plan.look};
+  const DecodePlan& how = plan.how;
   const bool d128 = p.cache.head_dim == 128;
-  if (how.wide || !by_rows)
+  if (how.wide || !plan.by_rows)
     return d128 ? launch_direct<128, 8, 2, true>(a, pr, how.ranks, stream, name)
                 : launch_direct<64, 8, 4, true>(a, pr, how.ranks, stream, name);
   return d128 ? launch_direct<128, 4, 2, true>(a, pr, 1, stream, name)
