@@ -870,7 +870,8 @@ SplitPlan split_plan(int64_t group, int64_t head_dim) {
 // KV heads of 128 dims, in a graph:
 // - items (row, KV head, pass) up to one per SM: 8 warps per CTA, and clusters while they too find an SM each
 //   (1 row of 1000 keys: 10.3 us with 4 warps, 8.4 with 8, 5.0 with clusters of 8; 8 rows of 1000: 10.6, 8.6 and
-//   7.2 with clusters of 2, but 11.9 with 512 CTAs in clusters of 8: a CTA that finds nothing to do still costs);
+//   7.2 with clusters of 2, but 11.9 with 512 CTAs in clusters of 8: a CTA that finds nothing to do still costs, so
+//   that a cluster is no larger than the context has steps for);
 // - more items: CTAs of 4 warps, three to an SM, one per item (256 rows of 50..150 keys: 26.9 us against 54.9 with 8
 //   warps; 64 rows of 64..2048: 52, as good);
 // - contexts that would keep one CTA busy for long: the split kernel. With equal lengths the two are even (64 rows of
@@ -892,11 +893,11 @@ DecodePlan decode_plan(int64_t rows, int64_t q_heads, int64_t kv_heads, int64_t 
   return p;
 }
 
-// Whether prompt rows go row by row, as in a decode call, instead of in tiles. A tile takes as long for one row as for
-// 128, but a row's keys are read for that row alone. With 16 query and 8 KV heads of 128 dims, tiles and rows: one prompt
-// of 13 rows 7.2 us and 3.9; 48 rows 7.4 and 4.4, 64 rows even; 4 rows behind 4000 keys 25.7 and 9.5; 16 rows behind 500
-// 13.7 and 6.6, behind 4000 25.9 and 21.4, behind 8000 32.6 and 38.9; 48 rows behind 1000 20.1 and 16.1, 24 behind 2000
-// 22.8 and 20.6. The host knows the table's columns only, not the rows' keys.
+// Whether a prompt call goes by rows, as a decode call does, instead of in tiles: a tile takes as long for one row as for
+// 128, but a pass over the keys serves no more than the eight columns of the products. With 16 query and 8 KV heads of 128
+// dims, tiles and rows: one prompt of 13 rows 7.2 us and 4.0, 64 rows 7.5 and 4.7, 200 rows 10.9 and 7.7, 300 rows 10.9 and
+// 12.8; 48 rows behind 1000 keys 20.1 and 9.7, 200 behind 1800 26.4 and 27.6; 16 behind 4000 25.9 and 14.9, 64 behind 6000
+// 28.9 and 32.0, 16 behind 24000 45.6 and 59.2. The host knows the table's columns only, not the rows' keys.
 struct PromptPlan {
   bool by_rows, look;
   int pack;
@@ -908,7 +909,8 @@ PromptPlan prompt_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64_t
   PromptPlan p;
   p.look = sequences <= 32 * kLookRounds && rows <= (int64_t(1) << 20);
   const int64_t units = kv_heads * ((group + kHeads - 1) / kHeads);
-  // the columns of several rows share a pass over the keys where that is long or the rows are many
+  // several rows' heads share a pass where it is long or the rows are many (16 rows behind 2000 keys 13.4 us alone and 10.6
+  // together; behind 500 6.7 and 7.5, 13 rows 3.9 and 4.6: finding the packs and fewer CTAs cost more than they save)
   const bool many = rows * units > 3 * sm_count() || capacity > 768;
   p.pack = many && p.look && group <= kHeads ? int(kHeads / group) : 1;
   // every sequence may end inside a pack

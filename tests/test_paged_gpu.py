@@ -366,6 +366,14 @@ def test_prompt_of_few_rows(ops, cuda, counts, starts, q, kv, d, page):
     check_prompt(ops, cuda, q, kv, d, page, counts, starts, lead=2, tail=1, strided=True)
 
 
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 6, 7, 8, 9])
+@pytest.mark.parametrize("kv,d", [(2, 64), (1, 128)])
+def test_prompt_rows_that_share_their_keys(ops, cuda, group, kv, d):
+    """Tables of more than 768 positions: 8 / group consecutive rows of a sequence make one item."""
+    check_prompt(ops, cuda, group * kv, kv, d, 16, [1, 7, 8, 9, 0, 17], [1000, 41, 0, 1009, 5, 333], lead=1, tail=2, strided=True)
+    check_prompt(ops, cuda, group * kv, kv, d, 16, [9, 12, 3], [-3, -20, 12], columns=64)   # padding inside of an item
+
+
 @pytest.mark.parametrize("count", [31, 33, 64, 127, 128, 129, 300])
 def test_prompt_of_few_rows_among_many_sequences(ops, cuda, count):
     counts, starts = [int(i % 3 == 1) + int(i == count - 1) for i in range(count)], [(7 * i) % 90 for i in range(count)]
