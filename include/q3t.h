@@ -448,7 +448,8 @@ int q3t_paged_decode_attention(const q3t_paged_decode* call, unsigned* status, v
  * row_offsets[s + 1] - 1 (int64 [sequences + 1], ascending, within 0 .. rows; sequences may be empty);
  * its i-th row has position start_positions[s] + i (start > 0: a chunk after a cached prefix; rows at
  * negative positions are left padding and give zeros) and sees keys 0 .. that position, all of which
- * the pool holds already and which are finite. Rows of no sequence are left as they are in out. Offsets
+ * the pool holds already and whose values are finite; a row that sees a key whose score is NaN or +inf is
+ * NaN. Rows of no sequence are left as they are in out. Offsets
  * that run backwards or leave 0 .. rows raise the bad-index bit; their sequence is skipped. The context that the
  * table's columns can hold helps to choose the form.
  * Otherwise as q3t_paged_decode_attention. */

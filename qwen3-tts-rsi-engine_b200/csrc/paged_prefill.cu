@@ -184,15 +184,22 @@ Q3T_DEV float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The largest of three; NaN where one of them is.
 Q3T_DEV float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+Q3T_DEV float max2(float a, float b) {
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
 }
 // 2^x of two values without the special-function unit, whose 16 results a cycle and SM the kernel is short of:
 // x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low bits), then 2^f on [-1/2, 1/2] as
 // 1 + a polynomial of degree 4 (fitted here for the least maximal relative error: 2^-18.4) and n added to the exponent.
-// From x = -127 down the result is exactly 0: f is 0 there, and 1.0's exponent becomes 0. Not for NaN.
+// From x = -127 down the result is exactly 0: f is 0 there, and 1.0's exponent becomes 0. NaN gives 0 too: such a row has
+// its NaN from its maximum.
 Q3T_DEV float2 exp2_poly(float2 x) {
   x.x = fmaxf(x.x, -127.f);
   x.y = fmaxf(x.y, -127.f);
@@ -514,9 +521,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 128; i += 2) mx[i / 2 & 3] = max3(mx[i / 2 & 3], s[i], s[i + 1]);
-        const float now = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-        if (__any_sync(0xffffffffu, now > top + 8.f || (top == -INFINITY && now > top))) {
-          const float to = fmaxf(top, now);
+        const float now = max2(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
+        // a NaN among the scores becomes the maximum, and with it the sum: the row has no value, wherever the NaN stands
+        if (__any_sync(0xffffffffu, !(now <= top + 8.f) && p < a.positions)) {  // rows past them hold anything
+          const float to = max2(top, now);
           const float f = to == top ? 1.f : exp2_fast(top - to);
           top = to;
           sum *= f;

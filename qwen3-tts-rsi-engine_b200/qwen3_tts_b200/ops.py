@@ -683,7 +683,8 @@ def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offse
 
     Sequence s owns query rows row_offsets[s] .. row_offsets[s + 1] - 1; its i-th row has position
     start_positions[s] + i (start > 0: a chunk after a cached prefix; negative positions are left padding and
-    give zeros) and sees keys 0 .. that position in the pages of page_table[s], which hold them already and finite.
+    give zeros) and sees keys 0 .. that position in the pages of page_table[s], which hold them already, the
+    values finite (a row that sees a key whose score is NaN or +inf is NaN).
     Rows that no sequence owns are left as they are in `out`, which must not overlap query or pages. The table's columns
     bound the context: with a view of fewer (page_table[:, :n]) few rows take the form for short contexts. `workspace`: as
     for paged_decode_attention."""

@@ -1,0 +1,54 @@
+"""The tiled form of the paged prompt attention: what the cases of the row form do not reach."""
+import pytest
+import torch
+
+from tests.paged_reference import BF16, Case, assert_within, attend, rng
+
+pytestmark = pytest.mark.gpu
+
+# Table widths with which prompts of hundreds of rows go in whole items, and in even ranges of key tiles
+WIDTHS = pytest.mark.parametrize("capacity", [None, 1 << 17], ids=["in-turn", "ranges"])
+HEADS = pytest.mark.parametrize("q,kv,d", [(16, 8, 128), (16, 8, 64), (12, 4, 64)])
+
+
+@pytest.fixture(scope="module")
+def ops(cuda):
+    from qwen3_tts_b200 import ops as _ops
+    return _ops
+
+
+def prompt(ops, cuda, case, query, rows, start=0, out=None):
+    """One sequence's `rows` rows from position `start` on; the status has to stay clear."""
+    keys, values, table = case.to(cuda)
+    out = torch.empty_like(query, device=cuda) if out is None else out
+    ops.paged_prefill_attention(query.to(cuda), keys, values, table, torch.tensor([0, rows], device=cuda),
+                                torch.tensor([start], device=cuda), out=out)
+    assert ops.read_status(cuda) == 0
+    return out.cpu()
+
+
+def case_of(length, kv, d, page, capacity, seed):
+    return Case([length], kv, d, page, seed=seed, columns=None if capacity is None else capacity // page)
+
+
+@WIDTHS
+@HEADS
+@pytest.mark.parametrize("score", [float("nan"), float("inf"), -float("inf")])
+def test_scores_that_are_not_finite_follow_the_formula(ops, cuda, q, kv, d, capacity, score):
+    """One key whose scores are NaN or +inf leaves no value to the rows that see it, wherever it stands, and does not
+    touch the others; one of -inf has weight 0."""
+    rows = 700
+    query = torch.randn(rows, q, d, generator=rng(3)).to(BF16)
+    query[..., 0] = query[..., 0].abs() + 0.25
+    for where in (1, 6, 7, 23, 64, 102, 103, 135, 383, 620):
+        case = case_of(rows, kv, d, 16, capacity, where)
+        case.keys[case.table[0, where // 16], :, where % 16, 0] = score
+        got = prompt(ops, cuda, case, query, rows)
+        keys, values = case.sequence(0, rows)
+        for r in {0, where - 1, where, where + 1, *range(where % 64, rows, 64), rows - 1}:
+            if r >= where and score != -float("inf"):
+                assert got[r].isnan().all(), f"key {where} row {r}"
+                continue
+            seen = [j for j in range(r + 1) if j != where]
+            want, bound = attend(query[r], keys[:, seen], values[:, seen], d ** -0.5)
+            assert_within(got[r], want, bound, f"key {where} row {r}")
