@@ -796,6 +796,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = warp_wait(&bars->takeover, i, a.status, kStatusFlagTimeout);
           int block = 0;
           if (!ok || !taken_over(&bars->response, block)) break;
+          fence_async_shared();  // every lane's read of the answer comes before the next one is written over it
+          __syncwarp();
           seg = find_tile(a, before, block / units, block % units, lane);
           if (seg.count > 0) {
             give(seg);

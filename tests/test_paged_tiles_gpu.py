@@ -52,3 +52,23 @@ def test_scores_that_are_not_finite_follow_the_formula(ops, cuda, q, kv, d, capa
             seen = [j for j in range(r + 1) if j != where]
             want, bound = attend(query[r], keys[:, seen], values[:, seen], d ** -0.5)
             assert_within(got[r], want, bound, f"key {where} row {r}")
+
+
+def test_every_item_is_taken_over_once(ops, cuda):
+    """Thousands of items of a few rows: a CTA takes over a hundred, one answer after the other in the same place."""
+    counts = [1 + i % 4 for i in range(2000)]
+    case = Case([8] * 16, 8, 128, 16)
+    keys, values, table = case.to(cuda)
+    rows = sum(counts)
+    query = torch.randn(rows, 16, 128, generator=rng(5)).to(BF16)
+    offsets = torch.tensor([0, *counts]).cumsum(0)
+    args = (query.to(cuda), keys, values, table.repeat(125, 1), offsets.to(cuda),
+            torch.tensor([i % 5 for i in range(2000)], device=cuda))
+    want = ops.paged_prefill_attention(*args, out=torch.full_like(args[0], float("nan")))
+    for _ in range(20):
+        assert torch.equal(ops.paged_prefill_attention(*args, out=torch.full_like(args[0], float("nan"))), want)
+    assert ops.read_status(cuda) == 0 and want.isfinite().all()
+    for s in range(0, 2000, 7):
+        r = int(offsets[s + 1]) - 1
+        keys, values = case.sequence(s % 16, s % 5 + counts[s])
+        assert_within(want[r], *attend(query[r], keys, values, 128 ** -0.5), f"sequence {s}")
