@@ -71,4 +71,12 @@ Q3T_HD int row_of(const int32_t* prefix, int rows, int64_t at, int64_t units) {
   return lo;
 }
 
+// Groups of 2^shift neighbours that `count` are in, and the least shift with which they are no more than `most`.
+Q3T_HD int groups_of(int64_t count, int shift) { return int((count + (int64_t(1) << shift) - 1) >> shift); }
+Q3T_HD int group_shift(int64_t count, int most) {
+  int shift = 0;
+  while (groups_of(count, shift) > most) ++shift;
+  return shift;
+}
+
 }  // namespace q3t

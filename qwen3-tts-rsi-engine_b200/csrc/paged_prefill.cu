@@ -43,9 +43,12 @@ constexpr int kThreads = 384;
 constexpr int kLeast = 4;          // key tiles of a part
 constexpr int kFixed = 2;          // what an item costs beside its key tiles, in key tiles
 constexpr int kAhead = 2;          // key tiles of an item that are still to be loaded when the next one is asked for
-constexpr int kPlanTiles = 2048;   // query tile pairs and sequences that a range plan holds
+constexpr int kPlanTiles = 2048;   // query tile pairs that a range plan holds, and entries of the numbers of whole items
 constexpr int kPlanSequences = 1024;
-constexpr int kPlanPairs = 1 << 22;  // kThreads times as many are counted in 32 bits
+// Query tile pairs that a sequence is counted with at most: kThreads sequences and all before them stay within 32 bits. A
+// sequence of more has 230 GB of queries and outputs at the least (4 rows of 43 heads of 64 dims a pair).
+constexpr int kMostPairs = 5 << 20;
+static_assert(int64_t(kThreads) * kMostPairs + (int64_t(1) << 28) / 4 + (1 << 20) < (int64_t(1) << 31), "32 bits");
 
 struct PrefillArgs {
   PageTable pages;
@@ -59,6 +62,7 @@ struct PrefillArgs {
   bool out_32;  // out is 32-byte aligned
   int parts;    // ranges, one per CTA; 0: whole items in turn
   int pairs;    // query tile pairs at most
+  int shift, groups;  // the CTA keeps the numbers behind every 2^shift sequences
   struct Segment* shared_segments;  // workspace: [parts][2], what a range left unfinished at its start (0) and end (1)
   float* partial;                   // workspace: [parts][2][D / 4][256 rows][4], then [256][2] (m, l)
   float scale_log2;
@@ -275,17 +279,20 @@ Q3T_DEV int key_tiles_of(const PrefillArgs& a, int64_t end) { return (keys_of(a,
 
 // Query tile pairs are numbered from the last of the last sequence backwards, so that those with the most keys
 // come first. One warp finds the sequence, rows and key tiles of number `index`; count 0: there is none. `before`: where the
-// CTA has it, the numbers of the sequences behind each, the last one first; without it 32 sequences are looked at at once.
+// CTA has it, the numbers behind every 2^shift sequences, the last one first, of which 32 at once are looked at; without it
+// all are (past 32 sequences that is too slow: 20000 of 2..6 rows, 8 KV heads, take 4.6 ms, and 169 with a look at all of
+// them for every item).
 Q3T_DEV Segment find_tile(const PrefillArgs& a, const int32_t* before, int index, int unit, int lane) {
   const int span = 2 * a.positions;
   Segment t = {};
-  int base = a.sequences - 1;
+  int base = a.sequences - 1, stop = 0;  // the first sequence to look at
   if (before != nullptr) {
-    const int i = row_of(before, a.sequences, index, 1);
-    base -= i;
+    const int i = row_of(before, a.groups, index, 1);
+    base -= i << a.shift;
+    stop = max(0, base + 1 - (1 << a.shift));
     index -= before[i];
   }
-  for (; base >= 0; base -= 32) {
+  for (; base >= stop; base -= 32) {
     const int s = base - lane;
     int n = 0, first = 0, tiles = 0;
     int64_t start = 0;
@@ -302,7 +309,6 @@ Q3T_DEV Segment find_tile(const PrefillArgs& a, const int32_t* before, int index
     }
     const unsigned hit = __ballot_sync(0xffffffffu, sum > index);
     if (hit == 0) {
-      if (before != nullptr) break;
       index -= __shfl_sync(0xffffffffu, sum, 31);
       continue;
     }
@@ -427,16 +433,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   int32_t* prefix = reinterpret_cast<int32_t*>(smem + M::kPlan);
   int32_t* before = nullptr;
   int pairs = 0;
-  if (a.parts > 0 || (a.sequences > 32 && a.sequences <= kPlanTiles && a.pairs <= kPlanPairs)) {
+  if (a.parts > 0 || a.sequences > 32) {
     before = a.parts > 0 ? prefix + kPlanTiles + 1 : prefix;
     const int span = 2 * a.positions;
     for (int s0 = 0; s0 < a.sequences; s0 += kThreads) {
       const int s = a.sequences - 1 - s0 - int(threadIdx.x);
       int first, n = s >= 0 ? rows_of(a, s, first) : 0, all;
       // offsets that run backwards may make sequences overlap: no more pairs are listed than rows in order can have
-      n = min((n + span - 1) / span, a.pairs);
-      const int sum = block_sum(n, bars->sums, warp, lane, all);
-      if (s >= 0) before[a.sequences - 1 - s] = min(pairs + sum - n, a.pairs);
+      n = min(min((n + span - 1) / span, a.pairs), kMostPairs);
+      const int sum = block_sum(n, bars->sums, warp, lane, all), i = a.sequences - 1 - s;
+      if (s >= 0 && (i & ((1 << a.shift) - 1)) == 0) before[i >> a.shift] = min(pairs + sum - n, a.pairs);
       pairs = min(pairs + all, a.pairs);
     }
     __syncthreads();
@@ -980,6 +986,8 @@ int launch_prefill_tiles(const q3t_paged_prefill& p, unsigned* status, void* str
   a.out_32 = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
   a.parts = plan.parts;
   a.pairs = int(plan.pairs);
+  a.shift = group_shift(p.sequences, kPlanTiles);  // 0 for ranges, whose sequences are fewer
+  a.groups = groups_of(p.sequences, a.shift);
   a.shared_segments = static_cast<Segment*>(p.workspace);
   a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + segment_bytes(plan.parts));
   const int64_t blocks = plan.parts > 0 ? plan.parts : plan.items;

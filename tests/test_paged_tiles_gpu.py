@@ -72,3 +72,33 @@ def test_every_item_is_taken_over_once(ops, cuda):
         r = int(offsets[s + 1]) - 1
         keys, values = case.sequence(s % 16, s % 5 + counts[s])
         assert_within(want[r], *attend(query[r], keys, values, 128 ** -0.5), f"sequence {s}")
+
+
+@pytest.mark.parametrize("count,period", [(2100, 301), (4097, 301), (50001, 331), (1 << 20, 48)])
+def test_sequences_by_the_thousand(ops, cuda, count, period):
+    """Sequence s is as s % period (its pages, length, start and queries), so that all rows are known from a few: up to
+    5 rows, one of the period none and one, where there are few sequences, several query tiles."""
+    counts = [(7 * i) % 6 for i in range(period)]
+    if count < 10000:
+        counts[period // 2] = 300
+    starts, lengths = [(5 * i) % 40 for i in range(period)], [n + 40 for n in counts]
+    case = Case(lengths, 1, 64, 16, seed=period)
+    first = torch.tensor([0, *counts]).cumsum(0)
+    small = torch.randn(int(first[-1]), 2, 64, generator=rng(period + 1)).to(BF16)
+    known = [attend(small[int(first[s]) + i], *case.sequence(s, starts[s] + i + 1), 0.125)
+             for s in range(period) for i in range(counts[s])]
+    want, bound = (torch.stack(x).to(cuda) for x in zip(*known))
+    kind = torch.arange(count, device=cuda) % period
+    many = torch.tensor(counts, device=cuda)[kind]
+    offsets = torch.cat((many.new_zeros(1), many.cumsum(0)))
+    rows = int(offsets[-1])
+    sequence = torch.repeat_interleave(torch.arange(count, device=cuda), many)
+    row = first.to(cuda)[kind[sequence]] + torch.arange(rows, device=cuda) - offsets[sequence]
+    keys, values, table = case.to(cuda)
+    query = small.to(cuda)[row]
+    got = ops.paged_prefill_attention(query, keys, values, table[kind], offsets, torch.tensor(starts, device=cuda)[kind],
+                                      out=torch.full_like(query, float("nan")))
+    assert ops.read_status(cuda) == 0
+    for r in range(0, rows, 1 << 19):
+        part, index = got[r:r + (1 << 19)], row[r:r + (1 << 19)]
+        assert ((part.double() - want[index]).abs() <= bound[index]).all(), f"rows from {r} on"
