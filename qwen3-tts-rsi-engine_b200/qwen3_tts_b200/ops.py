@@ -530,7 +530,8 @@ def decode_attention_qkv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin_
 
 # ------------------------------------------------------------------ paged key/value cache
 # These wrappers are called once or twice per layer and token, so each attribute is read once, in its cheap form
-# (get_device, identity of dtypes), and the arguments travel as one packed struct.
+# (get_device, identity of dtypes), and the arguments travel as one packed struct. The stride of a dim of one element is
+# of no matter and may be anything.
 _INT64, _INT32 = torch.int64, torch.int32
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
@@ -543,14 +544,16 @@ def _paged_cache(what: str, device: int, key_pages, value_pages, page_table):
         raise ValueError(f"{what}: expected CUDA tensors on one device")
     shape, stride = key_pages.shape, key_pages.stride()
     if (key_pages.dtype is not BF16 or value_pages.dtype is not BF16 or len(shape) != 4 or 0 in shape or value_pages.shape != shape
-            or value_pages.stride() != stride):
+            or (value_pages.stride() != stride and any(n > 1 and a != b for n, a, b in zip(shape, stride, value_pages.stride())))):
         raise ValueError(f"{what}: expected BF16 key and value pages [pages, Hkv, page_size, D], laid out alike")
     pages, heads, size, dim = shape
     page_stride, head_stride, row_stride, inner = stride
-    if inner != 1 or row_stride != dim or head_stride != size * dim:
+    if inner != 1 or row_stride != dim or (head_stride != size * dim and heads > 1):
         raise ValueError(f"{what}: pages must be dense [Hkv, page_size, D] blocks")
+    if pages == 1:
+        page_stride = heads * size * dim
     shape, stride = page_table.shape, page_table.stride()
-    if page_table.dtype is not _INT32 or len(shape) != 2 or stride[1] != 1:
+    if page_table.dtype is not _INT32 or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError(f"{what}: page table must be INT32 [sequences, columns] with unit inner stride")
     return (key_pages.data_ptr(), value_pages.data_ptr(), page_stride, pages, size, heads, dim, page_table.data_ptr(),
             stride[0], shape[0], shape[1], device)
@@ -565,13 +568,14 @@ def _paged_index(what: str, name: str, t, device: int, count: int) -> int:
 def _paged_query(what: str, query, dim: int, kv_heads: int, out, device: int):
     """(rows, query heads, row stride) of a query [rows, Hq, D] whose rows are dense."""
     shape, stride = query.shape, query.stride()
-    if (query.dtype is not BF16 or len(shape) != 3 or shape[2] != dim or stride[2] != 1 or stride[1] != dim
-            or shape[1] % kv_heads):
+    if (query.dtype is not BF16 or len(shape) != 3 or shape[2] != dim or stride[2] != 1
+            or (stride[1] != dim and shape[1] > 1) or shape[1] % kv_heads):
         raise ValueError(f"{what}: query must be BF16 [rows, Hq, D] with dense rows, Hq a multiple of Hkv")
     if out is not None and (out.get_device() != device or out.dtype is not BF16 or out.shape != shape
                             or not out.is_contiguous()):
         raise ValueError(f"{what}: out must be contiguous BF16 shaped like query")
-    return shape[0], shape[1], stride[0]
+    rows, heads = shape[0], shape[1]
+    return rows, heads, stride[0] if rows > 1 else heads * dim
 
 
 def _paged_workspace(what: str, need: int, workspace, device: int):
@@ -633,7 +637,7 @@ def paged_qk_norm_rope_kv(qkv, q_norm_weight, k_norm_weight, eps, cos_table, sin
         raise ValueError(f"{what}: query_out must be contiguous BF16 [rows, q_heads, head_dim]")
     if rows:
         _paged_call("q3t_paged_qk_norm_rope_kv", _lib.PAGED_WRITE.pack(
-            *cache, qkv.data_ptr(), stride[0], rows, q_heads, *norms, cos_table.data_ptr(), sin_table.data_ptr(),
+            *cache, qkv.data_ptr(), stride[0] if rows > 1 else shape[1], rows, q_heads, *norms, cos_table.data_ptr(), sin_table.data_ptr(),
             table_shape[0], rotary, positions, sequences or 0, query_out.data_ptr(), eps), device)
     return query_out
 
