@@ -696,6 +696,8 @@ def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offse
     device = query.get_device()
     cache = _paged_cache(what, device, key_pages, value_pages, page_table)
     _, _, _, _, size, kv_heads, dim, _, _, table_rows, columns, _ = cache
+    if out is None:
+        raise ValueError(f"{what}: out must be given (rows of no sequence are left as they are there)")
     rows, q_heads, row_stride = _paged_query(what, query, dim, kv_heads, out, device)
     sequences = start_positions.numel()
     starts = _paged_index(what, "start_positions", start_positions, device, sequences)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from qwen3_tts_b200 import _lib, ops
-from tests.test_paged_host import BF16, decode, index, no_launch, pool, prompt, table, write  # noqa: F401
+from tests.test_paged_host import BF16, FakeCuda, decode, index, no_launch, pool, prompt, table, write  # noqa: F401
 
 
 def odd(t, dim):
@@ -45,3 +45,10 @@ def test_a_dim_of_one_element_has_any_stride(entry, change, no_launch, monkeypat
     assert page_stride == heads * size * dim and (table_rows == 1 or table_stride == columns)
     rows, q_heads = fields[14:16]
     assert fields[13] == (q_heads + (2 * heads if entry is write else 0)) * dim
+
+
+def test_a_prompt_needs_an_output():
+    pages = [FakeCuda(pool()), FakeCuda(pool())]
+    with pytest.raises(ValueError, match="out must be given"):
+        ops.paged_prefill_attention(FakeCuda(zeros(9, 4, 64)), *pages, FakeCuda(table()), FakeCuda(index(4)),
+                                    FakeCuda(index(3)), out=None)
