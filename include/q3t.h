@@ -468,6 +468,10 @@ typedef struct {
 size_t q3t_paged_prefill_attention_workspace_bytes(int64_t rows, int64_t sequences, int64_t q_heads,
                                                    int64_t kv_heads, int64_t head_dim, int64_t context);
 int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsigned* status, void* stream);
+/* How a call of these sizes with a positive scale runs: 0 by rows, as a decode step; 1 in query tiles; 2 in query tiles
+ * whose keys are cut into even ranges. context: table_columns * page_size. */
+int q3t_paged_prefill_attention_form(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads,
+                                     int64_t head_dim, int64_t context);
 
 /* ------------------------------------------------------------------ sampling */
 

@@ -1010,6 +1010,14 @@ extern "C" size_t q3t_paged_prefill_attention_workspace_bytes(int64_t rows, int6
              : prefill_tiles_workspace(rows, sequences, q_heads, kv_heads, head_dim, context);
 }
 
+extern "C" int q3t_paged_prefill_attention_form(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads,
+                                                int64_t head_dim, int64_t context) {
+  if (rows < 1 || sequences < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || context < 1)
+    return fail(Q3T_EINVAL, "paged_prefill_attention_form: invalid geometry");
+  if (prompt_plan(rows, sequences, q_heads, kv_heads, context).by_rows || !prefill_tiles_supported(rows, context, 1.)) return 0;
+  return prefill_tiles_workspace(rows, sequences, q_heads, kv_heads, head_dim, context) > 0 ? 2 : 1;
+}
+
 extern "C" int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsigned* status, void* stream) {
   const char* name = "paged_prefill_attention";
   if (call == nullptr) return fail(Q3T_EINVAL, "%s: null pointer", name);
@@ -1022,7 +1030,7 @@ extern "C" int q3t_paged_prefill_attention(const q3t_paged_prefill* call, unsign
   const DeviceGuard guard(p.cache.device);
   if (!guard.ok()) return fail(Q3T_ECUDA, "%s: no such device", name);
   const PromptPlan plan = prompt_plan(p.rows, p.sequences, p.q_heads, p.cache.kv_heads, a.context);
-  if (!plan.by_rows && prefill_tiles_supported(p)) return launch_prefill_tiles(p, status, stream, name);
+  if (!plan.by_rows && prefill_tiles_supported(p.rows, a.context, p.scale)) return launch_prefill_tiles(p, status, stream, name);
   const PromptRows pr = {p.row_offsets, p.start_positions, int(p.sequences), plan.pack,
                          plan.pack > 1 ? int(255 / a.group + 1) : 0, int(plan.packs), plan.look};
   const DecodePlan& how = plan.how;

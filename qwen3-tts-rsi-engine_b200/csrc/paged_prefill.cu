@@ -948,10 +948,9 @@ PrefillPlan prefill_plan(int64_t rows, int64_t sequences, int64_t q_heads, int64
 
 namespace q3t {
 
-bool prefill_tiles_supported(const q3t_paged_prefill& p) {
-  const q3t_paged_cache& c = p.cache;
+bool prefill_tiles_supported(int64_t rows, int64_t capacity, double scale) {
   // an item of 2^26 keys takes a second, half of what a wait may take
-  return p.scale > 0. && p.scale < 1e30 && c.table_columns * c.page_size <= (int64_t(1) << 26) && p.rows < (int64_t(1) << 28);
+  return scale > 0. && scale < 1e30 && capacity <= (int64_t(1) << 26) && rows < (int64_t(1) << 28);
 }
 
 size_t prefill_tiles_workspace(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim,

@@ -91,6 +91,7 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "q3t_paged_decode_attention": (_i32, [_p, _p, _p]),
     "q3t_paged_prefill_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "q3t_paged_prefill_attention": (_i32, [_p, _p, _p]),
+    "q3t_paged_prefill_attention_form": (_i32, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "q3t_cdf_select": (_i32, [_p, _p, _p, _i64, _i64, _p]),
     "q3t_sample": (_i32, [_p, _i32, _i64, _p, _i64, _p, _p, _i64, _i64, _f32, _f32, _i64, _f32, _p, _i64, _u64,
                           _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p]),

@@ -681,6 +681,14 @@ def paged_prefill_attention_workspace_bytes(rows, sequences, q_heads, kv_heads, 
                                                                        context))
 
 
+def paged_prefill_attention_form(rows, sequences, q_heads, kv_heads, head_dim, context) -> str:
+    """How a prompt call of these sizes with a positive scale runs: "rows", "tiles" or "ranges" (of tiles)."""
+    form = _lib.load().q3t_paged_prefill_attention_form(rows, sequences, q_heads, kv_heads, head_dim, context)
+    if form < 0:
+        _lib.check(form, "q3t_paged_prefill_attention_form")
+    return ("rows", "tiles", "ranges")[form]
+
+
 def paged_prefill_attention(query, key_pages, value_pages, page_table, row_offsets, start_positions, *, out,
                             scale=None, workspace: Optional[torch.Tensor] = None):
     """Causal attention of packed prompts over a paged cache (q3t_paged_prefill_attention).

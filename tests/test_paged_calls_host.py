@@ -52,3 +52,13 @@ def test_a_prompt_needs_an_output():
     with pytest.raises(ValueError, match="out must be given"):
         ops.paged_prefill_attention(FakeCuda(zeros(9, 4, 64)), *pages, FakeCuda(table()), FakeCuda(index(4)),
                                     FakeCuda(index(3)), out=None)
+
+
+def test_the_form_of_a_prompt():
+    form = ops.paged_prefill_attention_form
+    assert form(13, 1, 8, 8, 64, 16) == "rows" and form(8191, 1, 32, 8, 128, 8192) == "tiles"
+    assert form(700, 1, 16, 8, 128, 1 << 17) == "ranges"
+    assert form(8191, 1, 32, 8, 128, (1 << 26) + 16) == "rows"     # more keys than the tiles count
+    for bad in ((0, 1, 8, 8, 64, 16), (13, 0, 8, 8, 64, 16), (13, 1, 4, 8, 64, 16), (13, 1, 8, 0, 64, 16), (13, 1, 8, 8, 64, 0)):
+        with pytest.raises(ValueError, match="geometry"):
+            form(*bad)
