@@ -28,6 +28,7 @@
 //   and l in the workspace, and a second, dependent launch joins the parts in the order of their keys (results repeat
 //   bit for bit). Parts are never smaller than kLeast tiles: short items move to one range whole.
 #include "common.cuh"
+#include "exp2_poly.cuh"
 #include "host.cuh"
 #include "paged.cuh"
 #include "paged_prefill.cuh"
@@ -198,24 +199,6 @@ Q3T_DEV float max2(float a, float b) {
   float c;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
   return c;
-}
-// 2^x of two values without the special-function unit, whose 16 results a cycle and SM the kernel is short of:
-// x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low bits), then 2^f on [-1/2, 1/2] as
-// 1 + a polynomial of degree 4 (fitted here for the least maximal relative error: 2^-18.4) and n added to the exponent.
-// From x = -127 down the result is exactly 0: f is 0 there, and 1.0's exponent becomes 0. NaN gives 0 too: such a row has
-// its NaN from its maximum.
-Q3T_DEV float2 exp2_poly(float2 x) {
-  x.x = fmaxf(x.x, -127.f);
-  x.y = fmaxf(x.y, -127.f);
-  const float2 n = add2(x, make_float2(12582912.f, 12582912.f));
-  const float2 f = add2(x, fma2(n, make_float2(-1.f, -1.f), make_float2(12582912.f, 12582912.f)));
-  float2 p = fma2(make_float2(0.009585323743522167f, 0.009585323743522167f), f,
-                  make_float2(0.05590662732720375f, 0.05590662732720375f));
-  p = fma2(p, f, make_float2(0.24024039506912231f, 0.24024039506912231f));
-  p = fma2(p, f, make_float2(0.6931241750717163f, 0.6931241750717163f));
-  p = fma2(p, f, make_float2(1.f, 1.f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(n.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(n.y) << 23)));
 }
 // Moves registers between the warpgroups: the CTA is launched with kThreads * 168, and 56 + 2 * 224 = 3 * 168.
 constexpr int kRegsLoad = 56, kRegsSoftmax = 224;
