@@ -15,8 +15,8 @@
 // row's maximum exceeds by at most 8 (powers of two), so O in TMEM is rescaled only when a maximum moves by more; O / l
 // does not depend on it. P's rounding to bf16 is that of a bf16 tensor product; S, m, l and O stay in fp32.
 //
-// One prompt of 8191 rows with 32 query and 8 KV heads of 128 dims: 435 us, 1265 TFLOP/s (512 us over seconds, under the
-// power cap). A pair of 128 x 128 key tiles takes 3150 cycles of which the tensor cores work 2080: scores, the first half of
+// One prompt of 8191 rows with 32 query and 8 KV heads of 128 dims: 510 us in a stream of calls, 1080 TFLOP/s, under the
+// power cap; 432 to 454 us in a short run (1270 to 1210). A pair of 128 x 128 key tiles takes 3150 cycles of which the tensor cores work 2080: scores, the first half of
 // the weights, their product and the next scores wait for one another, and there is no TMEM for a third tile.
 //
 // Work comes in one of two ways (the host picks by sizes):
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float2 x = fma2(make_float2(s[32 * quarter + 2 * i], s[32 * quarter + 2 * i + 1]), scale2, ref2);
-            if ((i & 7) == 3) {  // one in eight: 2 % (D = 128) to 8 % (64); one in four is no faster, one in two slower
+            if ((i & 7) == 3) {  // one in eight: 3 % for long prompts, -3 % for prompts of a few rows; one in four is no faster
               x = exp2_poly(x);
             } else {
               x.x = exp2_fast(x.x);

@@ -11,12 +11,13 @@
 // exchange between lanes and the norm only the D/16-lane sum. A lane takes HEADS heads of one kind of a row, whose
 // loads are all on their way before the first is used, and reads the row's positions, cos and sin once for them.
 //
-// 3500 rows of 16 + 2 * 8 heads of 128 dims: 13.1 us for 65.8 MB, 5.0 TB/s; 16000 rows 5.7 TB/s; 1 to 64 rows 2.3 us. The
-// same kernel that only copies takes 10.0 us for the 3500. With the weight, cos and sin unpacked and multiplied for every
-// head the kernel was bound by its instructions (276 for a warp's four heads, 60 % of the issue slots at 17 warps per
-// SM): 17.4 us; packed arithmetic on factors that four heads share 16.2, the dependent loads first 15.2, the rows kept
-// out of L1 13.1. Two or eight heads to a lane, a loop that fetches the next heads meanwhile (two of them in registers
-// leave fewer warps), and rows brought into shared memory by a copying warp were all slower.
+// 3887 rows of 16 + 2 * 8 heads of 128 dims: 15.1 us for 65.8 MB that are not in L2, 4.4 TB/s (13.1 where half of them are,
+// 10.2 where all are); 16000 rows 5.3 TB/s; 1 to 64 rows 1.9 to 2.4 us. The same kernel that only copies takes 11.7 us for
+// the 3887. With the weight, cos and sin unpacked and multiplied for every head the kernel was bound by its instructions;
+// packed arithmetic on factors that four heads share leaves 37 % of the issue slots in use, and the loads' latency is the
+// bound. Five CTAs an SM instead of what the registers would leave: 16.5 -> 15.1 us. Two or eight heads to a lane, a loop
+// that fetches the next heads meanwhile (two of them in registers leave fewer warps), and rows brought into shared memory
+// by a copying warp were all slower.
 #include "common.cuh"
 #include "host.cuh"
 #include "paged.cuh"
@@ -54,7 +55,8 @@ Q3T_DEV Words load8(const __nv_bfloat16* p) {
   const uint4 v = *reinterpret_cast<const uint4*>(p);
   return {{v.x, v.y, v.z, v.w}};
 }
-// The same for what is read once: it leaves L1 to the weights, cos and sin (3500 rows 15.2 -> 13.0 us).
+// The same for what is read once: it leaves L1 to the weights, cos and sin (3887 rows, of which L2 holds half, as behind
+// the projection that wrote them: 14.4 -> 13.1 us; with all of them in L2 no difference; from memory 14.6 -> 15.1).
 Q3T_DEV Words load8_once(const __nv_bfloat16* p) {
   Words v;
   asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -211,9 +213,9 @@ extern "C" int q3t_paged_qk_norm_rope_kv(const q3t_paged_write* call, unsigned* 
   a.kv_heads = int(c.kv_heads);
   a.rows = p.rows;
   a.status = status;
-  // few rows: a lane per head for the shortest chain (64 rows of 32 heads 2.4 us against 3.2 with four, 512 rows 3.4
-  // against 3.7); many: four heads to a lane share what a row needs once (1000 rows 5.1 us against 5.4, 3500 13.1
-  // against 16.5)
+  // few rows: a lane per head for the shortest chain (64 rows of 32 heads of 128 dims 2.1 us against 2.7 with four, 512
+  // rows 3.9 against 4.2); many: four heads to a lane share what a row needs once (1000 rows 5.9 us against 6.7, 3887 15.1
+  // against 16.9)
   const bool few = p.rows * heads <= 24576;
   if (c.head_dim == 128) return few ? launch_write<128, 1>(a, stream, name) : launch_write<128, 4>(a, stream, name);
   return few ? launch_write<64, 1>(a, stream, name) : launch_write<64, 4>(a, stream, name);

@@ -65,6 +65,27 @@ def test_scores_that_are_not_finite_follow_the_formula(ops, cuda, q, kv, d, capa
             assert_within(got[r], want, bound, f"key {where} row {r}")
 
 
+@pytest.mark.parametrize("q,kv,d", [(16, 8, 128), (16, 1, 64), (9, 1, 64)])
+@pytest.mark.parametrize("columns", [4, 60])
+@pytest.mark.parametrize("score", [float("nan"), float("inf"), -float("inf")])
+def test_scores_that_are_not_finite_by_rows(ops, cuda, q, kv, d, columns, score):
+    """The same where few rows go by rows, each alone or several in a pass over the keys."""
+    rows = 45
+    query = torch.randn(rows, q, d, generator=rng(3)).to(BF16)
+    query[..., 0] = query[..., 0].abs() + 0.25
+    for where in (1, 6, 16, 31, 40):
+        case = Case([rows], kv, d, 16, seed=where, columns=columns)
+        case.keys[case.table[0, where // 16], :, where % 16, 0] = score
+        got = prompt(ops, cuda, case, query, "rows")
+        keys, values = case.sequence(0, rows)
+        for r in range(rows):
+            if r >= where and score != -float("inf"):
+                assert got[r].isnan().all(), f"key {where} row {r}"
+                continue
+            seen = [j for j in range(r + 1) if j != where]
+            assert_within(got[r], *attend(query[r], keys[:, seen], values[:, seen], d ** -0.5), f"key {where} row {r}")
+
+
 def test_every_item_is_taken_over_once(ops, cuda):
     """Thousands of items of a few rows: a CTA takes over a hundred, one answer after the other in the same place."""
     counts = [1 + i % 4 for i in range(2000)]
