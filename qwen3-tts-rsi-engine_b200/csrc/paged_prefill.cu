@@ -485,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (const Segment* taken_segment = take(ok)) {
       const Segment& seg = *taken_segment;
       int key_tiles, seen0;  // of this query tile; keys that the row sees from the segment's first on
+      const bool real = p < min(a.positions, seg.count - t * a.positions) && h < seg.heads;  // others hold anything
       {
         key_tiles = seg.tiles[t];
         const int position = seg.position + t * a.positions + p;
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 128; i += 2) mx[i / 2 & 3] = max3(mx[i / 2 & 3], s[i], s[i + 1]);
         const float now = max2(max3(mx[0], mx[1], mx[2]), mx[3]) * a.scale_log2;
         // a NaN among the scores becomes the maximum, and with it the sum: the row has no value, wherever the NaN stands
-        if (__any_sync(0xffffffffu, !(now <= top + 8.f) && p < a.positions)) {  // rows past them hold anything
+        if (__any_sync(0xffffffffu, !(now <= top + 8.f) && real)) {
           const float to = max2(top, now);
           const float f = to == top ? 1.f : exp2_fast(top - to);
           top = to;
@@ -566,7 +567,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- O / l: each thread its row, a whole sector (16 dims) a store. A row without keys is 0; a maximum of +inf
         // leaves no value.
         const float inv = none ? 0.f : top == INFINITY ? NAN : 1.f / sum;
-        const bool real = p < min(a.positions, seg.count - t * a.positions) && h < seg.heads;
         __nv_bfloat16* to = a.out + ((int64_t(seg.row) + t * a.positions + p) * a.q_heads + seg.head0 + h) * D;
 #pragma unroll 1  // the code runs once an item: short is faster than unrolled, which waits for its instructions
         for (int c = 0; c < D / 32; ++c, to += 32) {

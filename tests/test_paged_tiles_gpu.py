@@ -291,3 +291,31 @@ def test_prompts_on_both_sides_of_the_limit_for_items(ops, cuda):
     for rows, by_rows in ((216, True), (220, False)):
         assert (ops.paged_prefill_attention_form(rows, 1, 16, 8, 128, 2048) == "rows") == by_rows
         check_prompt(ops, cuda, 16, 8, 128, 64, [rows], [1800], columns=32)
+
+
+@WIDTHS
+@HEADS
+def test_queries_that_are_not_finite_stay_in_their_rows(ops, cuda, q, kv, d, capacity):
+    """NaN and infinite queries, of a sequence or of nobody, in the tiles of others."""
+    case = Case([500, 400], kv, d, 16, columns=None if capacity is None else capacity // 16)
+    query = torch.randn(930, q, d, generator=rng(8)).to(BF16)
+    bad = [70, 71, 199, 444]
+    query[:10] = query[510:520] = query[920:] = float("nan")
+    for r, value in zip(bad, (float("nan"), float("inf"), -float("inf"), float("nan"))):
+        query[r, :, 3] = value
+    assert form_of(ops, query, case, 4) == form_for(capacity)
+    keys, values, table = case.to(cuda)
+    out = torch.full_like(query, 5.0, device=cuda)
+    ops.paged_prefill_attention(query.to(cuda), keys, values, table[[0, 0, 1, 1]].contiguous(),
+                                torch.tensor([10, 510, 520, 920, 920], device=cuda), torch.tensor([0, 0, 0, 0], device=cuda),
+                                out=out)
+    # rows 510 .. 519 belong to sequence 1 of four: finite keys, queries that are not
+    assert ops.read_status(cuda) == 0 and out[510:520].isnan().all()
+    assert (out[:10] == 5).all() and (out[920:] == 5).all()
+    for s, first, n in ((0, 10, 500), (1, 520, 400)):
+        for i in range(n):
+            if first + i in bad:
+                # a dim of +-inf scores +-inf by the key's sign: with both signs seen, some score is +inf
+                assert out[first + i].isnan().all()
+            elif i % 7 == 0 or first + i + 1 in bad or first + i - 1 in bad:
+                assert_within(out[first + i], *attend(query[first + i], *case.sequence(s, i + 1), d ** -0.5), f"row {first + i}")
